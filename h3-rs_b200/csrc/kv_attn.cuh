@@ -1,0 +1,83 @@
+// kv_attn.cuh -- shared by the attention kernels over the 8-bit paged cache (kv_common.cuh): their arguments, the rows
+// and keys of a slot, and the workspace that joins a slot's parts.
+//
+// With c = scale * log2(e) and keys j of page p, both scales leave the matrix products:
+//     t_j = c ks_p (q . kcode_j),   w_j = 2^(t_j + log2 vs_p - m),   m within 2^8 of the row's largest t_j + log2 vs_p
+//     O = sum_j w_j vcode_j,   l = sum_p (1 / vs_p) sum_{j in p} w_j,   out = O / l,   lse = ln 2 (m + log2 l)
+// so K and V enter the tensor cores as their codes, which 16-bit floats hold exactly, and one scale a page is applied
+// in f32.  What is rounded is w (f16) and the output; m, l, the scores and O are f32.
+//
+// q enters as f16: an f16 input as it is; a bf16 row times a power of two that brings its largest element into
+// [1, 2), which is exact but for elements below 2^-14 of the row's largest (their error is under 2^-25 of it).
+#pragma once
+#include "kv_common.cuh"
+
+namespace h3q {
+
+struct KvAttnArgs {
+  KvCache c;
+  KvSeqs s;
+  const uint16_t* q;
+  int64_t q_ts, q_hs;      // element strides of a token and a head
+  int kind;                // 1 f16, 2 bf16 (q and out)
+  int heads, per;          // query heads, and query heads to a kv head
+  const int32_t* lengths;  // [batch] tokens in the cache, the new ones included
+  int64_t window;          // 0: none
+  int causal;
+  float scale_log2;
+  uint16_t* out;           // [tokens, heads, dim]
+  float* lse;              // [tokens, heads] or null
+  int row_lo, row_hi;      // this launch takes the sequences whose rows (new tokens * per) are in (row_lo, row_hi]
+  int one;                 // every sequence of this launch has one slot, its own index
+  int64_t slots;
+  float* part;             // partial results of split items
+  int4* meta;              // [slots * kv_heads]: first part, parts
+};
+
+// What a slot stands for: `rows` query rows of sequence b, (token, head of the group) in that order, and the keys
+// [lo, hi) that any of them sees, lo a multiple of 16.
+struct KvSlot {
+  int b, s0, n, r0, rows;
+  int64_t len, lo, hi;
+};
+
+__device__ __forceinline__ bool kv_slot(const KvAttnArgs& a, int64_t slot, int b, int tile, KvSlot& t) {
+  const int s0 = kv_start(a.s, b), n = kv_start(a.s, b + 1) - s0;
+  const int64_t all = (int64_t)n * a.per;
+  t.rows = 0;
+  t.lo = t.hi = 0;
+  if (n <= 0 || all <= a.row_lo || all > a.row_hi) return false;
+  const int64_t r0 = (slot - (a.one ? b : kv_slot_base(a.s, b, a.per, tile, 1))) * tile;
+  if (r0 >= all) return false;
+  t.b = b;
+  t.s0 = s0;
+  t.n = n;
+  t.r0 = (int)r0;
+  t.rows = (int)(all - r0 < tile ? all - r0 : tile);
+  int64_t len = __ldg(a.lengths + b);
+  const int64_t most = a.s.width << a.c.page_log2;
+  len = len < 0 ? 0 : (len > most ? most : len);
+  t.len = len;
+  const int64_t first = len - n + r0 / a.per, last = len - n + (r0 + t.rows - 1) / a.per;
+  int64_t hi = a.causal ? (last + 1 < len ? last + 1 : len) : len;
+  int64_t lo = a.window > 0 && first + 1 > a.window ? first + 1 - a.window : 0;
+  hi = hi < 0 ? 0 : hi;
+  t.lo = lo & ~(int64_t)15;
+  t.hi = hi > t.lo ? hi : t.lo;
+  return true;
+}
+
+// the keys [lo, hi) that row r of the slot sees
+__device__ __forceinline__ void kv_row_keys(const KvAttnArgs& a, const KvSlot& t, int r, int64_t& lo, int64_t& hi) {
+  const int64_t pos = t.len - t.n + (t.r0 + r) / a.per;
+  hi = a.causal && pos + 1 < t.len ? pos + 1 : t.len;
+  lo = a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0;
+}
+
+// packed row and query head of row r of the slot, as an index into [tokens, heads]
+__device__ __forceinline__ int64_t kv_row_out(const KvAttnArgs& a, const KvSlot& t, int kvh, int r) {
+  const int rr = t.r0 + r;
+  return (int64_t)(t.s0 + rr / a.per) * a.heads + kvh * a.per + rr % a.per;
+}
+
+}  // namespace h3q

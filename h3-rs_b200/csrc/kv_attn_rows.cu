@@ -1,0 +1,568 @@
+// kv_attn_rows.cu -- attention over the 8-bit paged cache for few query rows to a kv head (one generated token, a few
+// drafted ones): bound by reading the cache once.
+//
+// The rows of a (sequence, kv head) -- its new tokens times the query heads that share the kv head -- are the 16 (or
+// 2 x 16) rows of mma.sync.m16n8k16 tiles, so the codes of a kv head are read once for all of them.  A warp takes 16
+// keys a step: 2 KB of K and of V codes arrive by cp.async in a ring of its own, are widened to f16 in registers and
+// go straight into the fragments.  The order of the head dim in Q.K and of the columns of O is free, so it is chosen to make
+// every lane's codes contiguous: lane (g, t) of the B fragment of K holds d = 32 t .. 32 t + 31 of key g, and of V
+// d = 16 g .. 16 g + 15 of keys 2t, 2t + 1, 2t + 8, 2t + 9.  The ring is swizzled so that both reads are free of
+// bank conflicts.
+//
+// Work is cut by keys, not by sequences: the units (128 keys of a sequence and kv head) of the whole call, in order,
+// are dealt to the CTAs in equal contiguous ranges.  A CTA's warps take the 16-key steps of a range in turn and
+// join their running (m, l, O) at its end; a (sequence, kv head) cut between CTAs goes through f32 parts in the
+// workspace, joined in order by a second kernel, so results do not depend on timing.
+#include <cstdint>
+#include <cuda_runtime.h>
+#include "kv_attn.cuh"
+#include "h3q_internal.h"
+
+namespace h3q {
+
+namespace {
+
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kUnit = kWarps * 16;  // keys of a unit
+constexpr float kMove = 8.f;        // log2 of the largest weight between moves of the running maximum
+
+template <int D, int MT>
+struct RowsCfg {
+  static constexpr int kStages = MT == 1 ? 3 : 6;
+  static constexpr int kStageBytes = 2 * 16 * D;           // K and V codes of 16 keys
+  static constexpr int kRing = kStages * kStageBytes;      // a warp's ring; its O of 16 MT rows fits there too
+  static constexpr int kQBytes = MT * 16 * D * 2;
+  static constexpr int kSmem = kWarps * kRing + kQBytes;
+  static_assert(kRing >= MT * 16 * D * 4, "the ring holds a warp's partial output");
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a) : "memory");
+  return r;
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// byte offset of 16-byte chunk `ch` of key row `row` in a 16-key tile of D bytes a row
+template <int D>
+__device__ __forceinline__ uint32_t tile_off(int row, int ch) {
+  if (D == 128) return (uint32_t)(row * 128 + ((ch ^ (row & 7)) << 4));
+  return (uint32_t)((row >> 1) * 128 + (((((row & 1) << 2) | ch) ^ (2 * ((row >> 1) & 3))) << 4));
+}
+
+// The units of the call in order, and this CTA's place in them: the units of kThreads slots at a time in shared
+// memory with their running sum.
+struct Sched {
+  int units[kThreads], pre[kThreads], seq[kThreads];
+  int warp_sum[kWarps];
+  int found;
+};
+
+template <int TILE>
+__device__ __forceinline__ int slot_units(const KvAttnArgs& a, int64_t slot, int& b) {
+  b = 0;
+  if (slot >= a.slots) return 0;
+  b = a.one ? (int)slot : kv_slot_seq(a.s, slot, a.per, TILE, 1);
+  KvSlot t;
+  if (!kv_slot(a, slot, b, TILE, t)) return 0;
+  return (int)((t.hi - t.lo + kUnit - 1) / kUnit);
+}
+
+// Fills `sc` with the slots from `base` on; returns the sum of their units.  All threads of the CTA.
+template <int TILE>
+__device__ __forceinline__ int sched_load(const KvAttnArgs& a, Sched& sc, int64_t base) {
+  __syncthreads();
+  int b;
+  const int u = slot_units<TILE>(a, base + threadIdx.x, b);
+  int x = u;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) sc.warp_sum[warp] = x;
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sc.warp_sum[w];
+    total += sc.warp_sum[w];
+  }
+  sc.units[threadIdx.x] = u;
+  sc.pre[threadIdx.x] = before + x - u;
+  sc.seq[threadIdx.x] = b;
+  __syncthreads();
+  return total;
+}
+
+template <int D, int CODES, int MT>
+__global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel(const KvAttnArgs a) {
+  using C = RowsCfg<D, MT>;
+  constexpr int TILE = MT * 16, NT = D / 8, KS = D / 16;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ Sched sc;
+  __shared__ float row_c[TILE];                   // c of the row: scale * log2 e and the power of two taken out of q
+  __shared__ float2 ml[kWarps][TILE];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  uint8_t* ring = smem + warp * C::kRing;
+  const uint32_t ring_u = smem_u32(ring);
+  const uint32_t q_u = smem_u32(smem + kWarps * C::kRing);
+
+  // the sum of all units, and this CTA's range of them
+  int64_t all = 0;
+  int here = 0;
+  for (int64_t base = 0; base < a.slots; base += kThreads) {
+    here = sched_load<TILE>(a, sc, base);
+    all += here;
+  }
+  all *= a.c.kv_heads;
+  // no more workers than units: every worker's range then holds a unit, and an item's parts are consecutive workers'
+  const int64_t workers = all < gridDim.x ? all : gridDim.x, w = blockIdx.x;
+  if (w >= workers) return;
+  int64_t x = all * w / workers;
+  const int64_t x_end = all * (w + 1) / workers;
+  // find x: the slots' units before `base`, then inside the chunk
+  int64_t base = 0, before = 0;
+  if (a.slots > kThreads) here = sched_load<TILE>(a, sc, 0);
+  while (x >= (before + here) * a.c.kv_heads) {
+    before += here;
+    base += kThreads;
+    here = sched_load<TILE>(a, sc, base);
+  }
+  {
+    const int64_t p0 = (before + sc.pre[threadIdx.x]) * a.c.kv_heads;
+    if (x >= p0 && x < p0 + (int64_t)sc.units[threadIdx.x] * a.c.kv_heads) sc.found = threadIdx.x;
+  }
+  __syncthreads();
+  int li = sc.found;
+  bool first_segment = true;
+
+  while (true) {
+    // ---------------------------------------------------------------- the segment: units [u0, u1) of (slot, kvh)
+    const int units = sc.units[li];
+    const int64_t item0 = (before + sc.pre[li]) * a.c.kv_heads;  // units before the slot
+    const int kvh = (int)((x - item0) / units);
+    const int u0 = (int)((x - item0) % units);
+    const int u1 = (int)(x_end - x < units - u0 ? u0 + (x_end - x) : units);
+    const bool whole = u0 == 0 && u1 == units;
+    KvSlot sl;
+    kv_slot(a, base + li, sc.seq[li], TILE, sl);
+    const int64_t key0 = sl.lo + (int64_t)u0 * kUnit;
+    const int64_t key1 = sl.lo + (int64_t)u1 * kUnit < sl.hi ? sl.lo + (int64_t)u1 * kUnit : sl.hi;
+    const int steps_all = (int)((key1 - key0 + 15) / 16);
+    const int steps = steps_all > warp ? (steps_all - warp + kWarps - 1) / kWarps : 0;
+    const int64_t group0 = key0 / 16 + warp;
+
+    auto page_of = [&](int st) -> int64_t {
+      return st < steps ? kv_page(a.c, a.s, sl.b, ((group0 + (int64_t)st * kWarps) * 16) >> a.c.page_log2) : -1;
+    };
+    auto issue = [&](int st, int64_t page) {
+      if (st < steps) {
+        const bool there = page >= 0;
+        const int64_t key = (group0 + (int64_t)st * kWarps) * 16;
+        const int64_t off =
+            there ? ((page * a.c.kv_heads + kvh) * a.c.page + (key & (a.c.page - 1))) * D : 0;
+        const uint32_t dst = ring_u + (st % C::kStages) * C::kStageBytes;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const int ch = lane + 32 * i;
+          const uint32_t o = tile_off<D>(ch / (D / 16), ch % (D / 16));
+          cp16(dst + o, a.c.k + off + ch * 16, there);
+          cp16(dst + 16 * D + o, a.c.v + off + ch * 16, there);
+        }
+      }
+      cp_commit();
+    };
+
+    int64_t pages[C::kStages];  // pages of the steps in flight; [0]: the step consumed next
+#pragma unroll
+    for (int i = 0; i < C::kStages; ++i) pages[i] = page_of(i);
+#pragma unroll
+    for (int i = 0; i < C::kStages - 1; ++i) issue(i, pages[i]);
+
+    // ---------------------------------------------------------------- q: f16 in the order of the A fragments
+    for (int r = warp; r < TILE; r += kWarps) {
+      float f[D / 32];
+      float mx = 0.f;
+      const bool in = r < sl.rows;
+      const int rr = sl.r0 + r;
+      const uint16_t* src =
+          a.q + (int64_t)(sl.s0 + rr / a.per) * a.q_ts + (int64_t)(kvh * a.per + rr % a.per) * a.q_hs;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const uint16_t v = in ? __ldg(src + lane + 32 * i) : (uint16_t)0;
+        f[i] = a.kind == 1 ? h2f(v) : bf2f(v);
+        mx = fmaxf(mx, fabsf(f[i]));
+      }
+      float c = a.scale_log2;
+      if (a.kind == 2) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        if (mx > 0.f && mx < INFINITY) {
+          const int e = ilogbf(mx);
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) f[i] = scalbnf(f[i], -e);
+          c = scalbnf(c, e);
+        }
+      }
+      if (lane == 0) row_c[r] = c;
+      // element d of the row: lane t = d / (D / 4) of the quad, its element e = d % (D / 4); pair of k-steps e / 8
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const int d = lane + 32 * i, tt = d / (D / 4), e = d % (D / 4);
+        const int mt = r >> 4, half = (r >> 3) & 1, gg = r & 7;
+        const uint32_t o = (uint32_t)((((mt * (D / 32) + e / 8) * 2 + half) * 32 + gg * 4 + tt) * 16 + (e % 8) * 2);
+        asm volatile("st.shared.b16 [%0], %1;" ::"r"(q_u + o), "h"(f2h(f[i])) : "memory");
+      }
+    }
+    __syncthreads();
+
+    float o_acc[MT][NT][4];
+    float m_run[MT][2], l_run[MT][2], cr[MT][2];
+    int rlo[MT][2], rhi[MT][2];  // the row's keys, relative to key0
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o_acc[mt][j][e] = 0.f;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int r = mt * 16 + hf * 8 + g;
+        m_run[mt][hf] = -INFINITY;
+        l_run[mt][hf] = 0.f;
+        cr[mt][hf] = row_c[r];
+        int64_t lo = 0, hi = 0;
+        if (r < sl.rows) kv_row_keys(a, sl, r, lo, hi);
+        lo -= key0;
+        hi -= key0;
+        rlo[mt][hf] = (int)(lo < 0 ? 0 : (lo > 0x3fffffff ? 0x3fffffff : lo));
+        rhi[mt][hf] = (int)(hi < 0 ? 0 : (hi > 0x3fffffff ? 0x3fffffff : hi));
+      }
+    }
+    // keys of this segment that every row sees need no mask
+    const int64_t pos0 = sl.len - sl.n + sl.r0 / a.per, pos1 = sl.len - sl.n + (sl.r0 + sl.rows - 1) / a.per;
+    const int64_t all_hi = (a.causal && pos0 + 1 < sl.len ? pos0 + 1 : sl.len) - key0;
+    const int64_t all_lo = (a.window > 0 && pos1 + 1 > a.window ? pos1 + 1 - a.window : 0) - key0;
+
+    for (int st = 0; st < steps; ++st) {
+      cp_wait<C::kStages - 2>();
+      __syncwarp();
+      issue(st + C::kStages - 1, pages[C::kStages - 1]);
+      const int64_t page = pages[0];
+#pragma unroll
+      for (int i = 0; i + 1 < C::kStages; ++i) pages[i] = pages[i + 1];
+      pages[C::kStages - 1] = page_of(st + C::kStages);
+      if (page < 0) continue;
+      const float ks = __ldg(a.c.k_scale + page * a.c.kv_heads + kvh);
+      const float vs = fmaxf(__ldg(a.c.v_scale + page * a.c.kv_heads + kvh), kKvScaleFloor);
+      const uint32_t kt = ring_u + (st % C::kStages) * C::kStageBytes, vt = kt + 16 * D;
+      const int rel = (warp + st * kWarps) * 16;  // first key of the step, relative to key0
+
+      // ------------------------------------------------------------ S = Q K^T: two 8-key tiles
+      float s[MT][2][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
+#pragma unroll
+      for (int sp = 0; sp < KS / 2; ++sp) {  // two k-steps: 8 codes a lane and key
+        uint32_t kw[2][2];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          const int row = nt * 8 + g, byte = t4 * (D / 4) + sp * 8;
+          const uint2 r = lds64(kt + tile_off<D>(row, byte >> 4) + (byte & 8));
+          kw[nt][0] = r.x;
+          kw[nt][1] = r.y;
+        }
+        uint32_t b[2][4];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          kv_decode4<CODES>(kw[nt][0], b[nt][0], b[nt][1]);
+          kv_decode4<CODES>(kw[nt][1], b[nt][2], b[nt][3]);
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const uint4 qa = lds128(q_u + (uint32_t)((((mt * (D / 32) + sp) * 2 + 0) * 32 + lane) * 16));
+          const uint4 qb = lds128(q_u + (uint32_t)((((mt * (D / 32) + sp) * 2 + 1) * 32 + lane) * 16));
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) {
+            mma16816(s[mt][nt], qa.x, qb.x, qa.y, qb.y, b[nt][0], b[nt][1]);
+            mma16816(s[mt][nt], qa.z, qb.z, qa.w, qb.w, b[nt][2], b[nt][3]);
+          }
+        }
+      }
+
+      // ------------------------------------------------------------ weights
+      const float lv = kv_lg2(vs), iv = __fdividef(1.f, vs);
+      const bool edge = rel < all_lo || rel + 16 > all_hi;
+      uint32_t pa[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        float tv[2][4];  // [row half][key]
+        bool up = false;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const float ck = cr[mt][hf] * ks;
+          float mx = -INFINITY;
+#pragma unroll
+          for (int k4 = 0; k4 < 4; ++k4) {
+            float v = __fmaf_rn(s[mt][k4 >> 1][hf * 2 + (k4 & 1)], ck, lv);
+            if (edge) {
+              const int key = rel + (k4 >> 1) * 8 + 2 * t4 + (k4 & 1);
+              v = key >= rlo[mt][hf] && key < rhi[mt][hf] ? v : -INFINITY;
+            }
+            tv[hf][k4] = v;
+            mx = fmaxf(mx, v);
+          }
+          up |= mx > m_run[mt][hf] + kMove;
+        }
+        if (__any_sync(0xffffffffu, up)) {  // rare after the first steps: move the maximum of the rows that need it
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            float mx = fmaxf(fmaxf(tv[hf][0], tv[hf][1]), fmaxf(tv[hf][2], tv[hf][3]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            if (mx > m_run[mt][hf] + kMove) {
+              const float f = kv_ex2(m_run[mt][hf] - mx);  // 0 from -inf
+              m_run[mt][hf] = mx;
+              l_run[mt][hf] *= f;
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                o_acc[mt][j][2 * hf] *= f;
+                o_acc[mt][j][2 * hf + 1] *= f;
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const float m = m_run[mt][hf] == -INFINITY ? 0.f : m_run[mt][hf];
+          float p[4];
+#pragma unroll
+          for (int k4 = 0; k4 < 4; ++k4) p[k4] = kv_ex2(tv[hf][k4] - m);
+          l_run[mt][hf] = __fmaf_rn((p[0] + p[1]) + (p[2] + p[3]), iv, l_run[mt][hf]);
+          pa[mt][hf] = kv_pack_f16(p[0], p[1]);
+          pa[mt][2 + hf] = kv_pack_f16(p[2], p[3]);
+        }
+      }
+
+      // ------------------------------------------------------------ O += W V
+      const int64_t left = sl.len - (key0 + rel);  // keys of this step that the sequence has
+#pragma unroll
+      for (int jq = 0; jq < NT / 4; ++jq) {  // 4 column tiles: one word of each of the lane's four keys
+        uint32_t vw[4];
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4) {
+          const int row = (k4 >> 1) * 8 + 2 * t4 + (k4 & 1), byte = g * (D / 8) + jq * 4;
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(vw[k4]) : "r"(vt + tile_off<D>(row, byte >> 4) + (byte & 12)) : "memory");
+          if (left < 16 && row >= left) vw[k4] = 0;  // what lies behind the last token may be any bits
+        }
+        uint32_t b0[4], b1[4];
+        kv_decode4<CODES>(prmt(vw[0], vw[1], 0x5140), b0[0], b0[1]);
+        kv_decode4<CODES>(prmt(vw[0], vw[1], 0x7362), b0[2], b0[3]);
+        kv_decode4<CODES>(prmt(vw[2], vw[3], 0x5140), b1[0], b1[1]);
+        kv_decode4<CODES>(prmt(vw[2], vw[3], 0x7362), b1[2], b1[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            mma16816(o_acc[mt][jq * 4 + j], pa[mt][0], pa[mt][1], pa[mt][2], pa[mt][3], b0[j], b1[j]);
+      }
+    }
+    cp_wait<0>();
+    __syncwarp();
+
+    // ---------------------------------------------------------------- join the warps
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        float l = l_run[mt][hf];
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (t4 == 0) ml[warp][mt * 16 + hf * 8 + g] = make_float2(m_run[mt][hf], l);
+      }
+    __syncthreads();
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int r = mt * 16 + hf * 8 + g;
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) m = fmaxf(m, ml[i][r].x);
+        const float f = m_run[mt][hf] == -INFINITY ? 0.f : kv_ex2(m_run[mt][hf] - m);
+        // lane t holds d = t (D / 4) .. of the row: columns 2t and 2t + 1 of the tiles
+#pragma unroll
+        for (int hc = 0; hc < 2; ++hc)
+#pragma unroll
+          for (int jq = 0; jq < NT / 4; ++jq) {
+            const int ch = t4 * (D / 16) + hc * (D / 32) + jq;  // 16-byte chunk of the row
+            const uint32_t o = (uint32_t)(r * D * 4 + ((ch ^ ((t4 * 2 + (r & 1)) & 7)) << 4));
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = o_acc[mt][jq * 4 + j][2 * hf + hc] * f;
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(ring_u + o), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                         "f"(v[3])
+                         : "memory");
+          }
+      }
+    __syncthreads();
+    const int part_slot = (int)(w * 2 + (first_segment ? 0 : 1));
+    float* part = a.part + (int64_t)part_slot * TILE * (D + 2);
+    for (int i = threadIdx.x; i < TILE * (D / 4); i += kThreads) {
+      const int r = i / (D / 4), ch = i % (D / 4), tt = ch / (D / 16);
+      if (r >= sl.rows) continue;
+      const uint32_t o = (uint32_t)(r * D * 4 + ((ch ^ ((tt * 2 + (r & 1)) & 7)) << 4));
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) m = fmaxf(m, ml[k][r].x);
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float2 e = ml[k][r];
+        l += e.x == -INFINITY ? 0.f : e.y * kv_ex2(e.x - m);
+      }
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(smem + k * C::kRing + o);
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+      }
+      if (whole) {
+        const int64_t ro = kv_row_out(a, sl, kvh, r);
+        const float inv = l > 0.f ? __fdiv_rn(1.f, l) : (l == 0.f ? 0.f : l);  // a NaN goes through
+        uint2 o2;
+        o2.x = kv_pack(sum.x * inv, sum.y * inv, a.kind);
+        o2.y = kv_pack(sum.z * inv, sum.w * inv, a.kind);
+        *reinterpret_cast<uint2*>(a.out + ro * D + ch * 4) = o2;
+        if (a.lse && ch == 0) a.lse[ro] = l == 0.f ? -INFINITY : 0.6931471805599453f * (m + log2f(l));
+      } else {
+        *reinterpret_cast<float4*>(part + (int64_t)r * D + ch * 4) = sum;
+        if (ch == 0) *reinterpret_cast<float2*>(part + (int64_t)TILE * D + 2 * r) = make_float2(m, l);
+      }
+    }
+    if (u0 == 0 && threadIdx.x == 0) {
+      // who holds the rest: the worker of unit y is the last one whose range begins at or before y
+      const int64_t y = item0 + (int64_t)kvh * units + units - 1;
+      const int64_t w1 = ((y + 1) * workers - 1) / all;
+      a.meta[(base + li) * a.c.kv_heads + kvh] = make_int4(part_slot, (int)(w1 - w) + 1, (int)w, 0);
+    }
+    first_segment = false;
+    x += u1 - u0;
+    if (x >= x_end) break;
+    __syncthreads();  // the rings, q and the statistics are read: the next segment may fill them
+    if (x >= item0 + (int64_t)units * a.c.kv_heads) {  // the next slot that has units
+      ++li;
+      while (true) {
+        while (li < kThreads && sc.units[li] == 0) ++li;
+        if (li < kThreads) break;
+        before += here;
+        base += kThreads;
+        here = sched_load<TILE>(a, sc, base);
+        li = 0;
+      }
+    }
+  }
+}
+
+// Joins the parts of the items that were cut, in their order, and writes the rows of slots without keys: a warp a row.
+template <int D, int MT>
+__global__ void __launch_bounds__(256) kv_attn_join_kernel(const KvAttnArgs a) {
+  constexpr int TILE = MT * 16, E = D / 32;
+  const int64_t item = blockIdx.x;
+  const int64_t slot = item / a.c.kv_heads;
+  const int kvh = (int)(item % a.c.kv_heads);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b = a.one ? (int)slot : kv_slot_seq_warp(a.s, slot, a.per, TILE, 1);
+  KvSlot sl;
+  if (!kv_slot(a, slot, b, TILE, sl)) return;
+  const bool none = sl.hi <= sl.lo;
+  int4 meta = make_int4(0, 0, 0, 0);
+  if (!none) {
+    meta = a.meta[item];
+    if (meta.y <= 1) return;  // written whole
+  }
+  for (int r = warp; r < sl.rows; r += 8) {
+    float m = -INFINITY, l = 0.f, o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int i = 0; i < meta.y; ++i) {  // later parts are their worker's first segment
+      const float* part = a.part + (int64_t)(i == 0 ? meta.x : 2 * (meta.z + i)) * TILE * (D + 2);
+      const float2 e2 = *reinterpret_cast<const float2*>(part + (int64_t)TILE * D + 2 * r);
+      if (e2.x == -INFINITY) continue;
+      const float mn = fmaxf(m, e2.x);
+      const float f = m == -INFINITY ? 0.f : kv_ex2(m - mn), f2 = kv_ex2(e2.x - mn);
+      l = l * f + e2.y * f2;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = o[e] * f + part[(int64_t)r * D + lane * E + e] * f2;
+      m = mn;
+    }
+    const int64_t ro = kv_row_out(a, sl, kvh, r);
+    const float inv = l > 0.f ? __fdiv_rn(1.f, l) : (l == 0.f ? 0.f : l);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + ro * D + lane * E);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) dst[e] = kv_pack(o[2 * e] * inv, o[2 * e + 1] * inv, a.kind);
+    if (a.lse && lane == 0) a.lse[ro] = l == 0.f ? -INFINITY : 0.6931471805599453f * (m + log2f(l));
+  }
+}
+
+template <int D, int CODES, int MT>
+cudaError_t launch_rows(KvAttnArgs a, cudaStream_t st) {
+  using C = RowsCfg<D, MT>;
+  auto kern = kv_attn_rows_kernel<D, CODES, MT>;
+  static bool ready[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!ready[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+    ready[dev] = true;
+  }
+  kern<<<(unsigned)(sm_count(dev) * (MT == 1 ? 2 : 1)), kThreads, C::kSmem, st>>>(a);
+  if (const cudaError_t e = cudaGetLastError()) return e;
+  kv_attn_join_kernel<D, MT><<<(unsigned)(a.slots * a.c.kv_heads), 256, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+size_t kv_attn_rows_part_bytes(int dim, int tile) { return (size_t)sm_count(0) * 4 * tile * (dim + 2) * 4; }
+
+// tile: 16 or 32 rows
+cudaError_t launch_kv_attn_rows(const KvAttnArgs& a, int tile, cudaStream_t st) {
+#define H3Q_KV_A(DD, CC, MM) \
+  if (a.c.dim == DD && a.c.codes == CC && tile == MM * 16) return launch_rows<DD, CC, MM>(a, st);
+  H3Q_KV_A(64, 0, 1) H3Q_KV_A(64, 1, 1) H3Q_KV_A(128, 0, 1) H3Q_KV_A(128, 1, 1)
+  H3Q_KV_A(64, 0, 2) H3Q_KV_A(64, 1, 2) H3Q_KV_A(128, 0, 2) H3Q_KV_A(128, 1, 2)
+#undef H3Q_KV_A
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace h3q

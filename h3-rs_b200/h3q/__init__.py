@@ -45,6 +45,14 @@ class HostLinear(ctypes.Structure):
                 ("k", ctypes.c_int64), ("swiglu", ctypes.c_int), ("rotate", ctypes.c_int)]
 
 
+class KvCacheDesc(ctypes.Structure):
+    """h3q_kv_cache: the 8-bit paged key / value cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("pages", ctypes.c_int64), ("kv_heads", ctypes.c_int64),
+                ("page", ctypes.c_int), ("head_dim", ctypes.c_int), ("codes", ctypes.c_int)]
+
+
+KV_INT8, KV_E4M3 = 0, 1
 FMT_DENSE, FMT_INT8, FMT_NVFP4 = 0, 1, 2
 ATTN_SCALE_TOKEN, ATTN_SCALE_BLOCK128, ATTN_PV_F16, ATTN_PV_BF16 = 0, 1, 0, 2
 PATH_GEMM_S8, PATH_INT8_LINEAR, PATH_ROTATE_FUSED, PATH_ROTATE_SEPARATE, PATH_SWIGLU_FUSED, PATH_SWIGLU_AFTER = (
@@ -142,6 +150,12 @@ SIGNATURES = {
     "h3q_attn_kmean": (_int, [_vp, _i64, _i64, _vp, _vp, _sz, _vp]),
     "h3q_attn_quant_heads": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _int, _vp]),
     "h3q_attn_v_layout": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _int, _vp]),
+    "h3q_kv_write": (_int, [ctypes.POINTER(KvCacheDesc), _vp, _i64, _i64, _vp, _i64, _i64, _int, _i64, _vp, _i64, _vp,
+                            _vp, _i64, _vp]),
+    "h3q_kv_read": (_int, [ctypes.POINTER(KvCacheDesc), _vp, _i64, _vp, _vp, _i64, _i64, _vp, _vp, _int, _vp]),
+    "h3q_kv_attention_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _int, _i64]),
+    "h3q_kv_attention": (_int, [ctypes.POINTER(KvCacheDesc), _vp, _int, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64,
+                                _i64, ctypes.c_float, _int, _i64, _vp, _vp, _vp, _sz, _vp]),
     "h3q_attention_core": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp]),
 }
 

@@ -552,6 +552,69 @@ h3q_status h3q_gemm_s8_static(const uint16_t* x, const int8_t* w, const float* w
  * *code) when a kernel of an h3q_gemm_s8_static call gave up a bounded wait since the last read, else H3Q_OK. */
 h3q_status h3q_gemm_s8_static_status(int device, int* code);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * An 8-bit paged key / value cache: written as tokens arrive, read back, and attended to in place.  No counterpart
+ * in the reference, whose text encoder and DiT see their whole sequence in every call.
+ *
+ * The cache is a pool of pages.  Page p of kv head h holds `page` tokens of head_dim codes contiguously and one f32
+ * scale for K and one for V: k and v are [pages, kv_heads, page, head_dim] codes (int8 or e4m3), k_scale and v_scale
+ * [pages, kv_heads], value = code * scale.  Sequence b's tokens i * page .. are in page page_table[b, i] (int32
+ * [batch, table_width]); an entry outside [0, pages) names no page.  This build handles head_dim 64 and 128 and pages
+ * of 16, 32, 64 or 128 tokens.
+ *
+ * The packed tokens of a call belong to its sequences by `starts` (int32 [batch + 1], ascending from 0 to tokens;
+ * a sequence may have none), or evenly where starts is NULL.  page_table, past, lengths, first and starts are in
+ * device memory and never read by the host: a call can be captured in a graph and replayed on other values.  Two
+ * sequences may share a page that neither of them writes. */
+enum { H3Q_KV_INT8 = 0, H3Q_KV_E4M3 = 1 };
+typedef struct h3q_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t pages, kv_heads;
+  int page, head_dim;
+  int codes; /* H3Q_KV_* */
+} h3q_kv_cache;
+
+/* Appends k and v (rows [tokens, kv_heads, head_dim] of `kind`, unit stride inside a head, strides in elements) behind
+ * the past[b] (int32) tokens of each sequence.  For each page and head that gets new rows x, with top = 127 (int8) or
+ * 448 (e4m3) and amax over the finite elements of x:
+ *   s = max(old scale, amax * (1 / top), 1e-30)   (no old scale where the page's first token is among the new ones)
+ *   code = round(x * (1 / s)); where s grew, the page's older codes become round(code * (old / s))
+ * (round: to nearest even in the code type.)  An infinity is stored as +-top, a NaN as 0.  Tokens whose page is not there are dropped. */
+h3q_status h3q_kv_write(const h3q_kv_cache* cache, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                        const void* v, int64_t v_token_stride, int64_t v_head_stride, int kind, int64_t tokens,
+                        const int32_t* page_table, int64_t table_width, const int32_t* past, const int32_t* starts,
+                        int64_t batch, void* stream);
+
+/* Reads tokens first[b] .. first[b] + starts[b + 1] - starts[b] - 1 of each sequence (first NULL: from 0) into dense
+ * k_out and v_out [tokens, kv_heads, head_dim] of `kind`: code * scale, rounded once.  Tokens whose page is not
+ * there read as zeros. */
+h3q_status h3q_kv_read(const h3q_kv_cache* cache, const int32_t* page_table, int64_t table_width, const int32_t* first,
+                       const int32_t* starts, int64_t batch, int64_t tokens, void* k_out, void* v_out, int kind,
+                       void* stream);
+
+/* Workspace bytes h3q_kv_attention needs for the same arguments. */
+size_t h3q_kv_attention_workspace_size(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int head_dim,
+                                       int64_t max_new);
+
+/* Attention of the newest tokens of each sequence to its cache: out[t, h] = softmax(scale * q[t, h] . K) V over the
+ * sequence's first lengths[b] (int32) tokens, which include the new ones (write them first).  Query i of the n new
+ * tokens of a sequence stands at position lengths[b] - n + i; with `causal` it sees keys up to its own position, with
+ * window > 0 (causal only) the last `window` of those.  A row that sees no key gives zeros.  heads is a multiple of kv_heads: query
+ * head h reads kv head h / (heads / kv_heads).  q is [tokens, heads, head_dim] of `kind` (f16 or bf16; strides in
+ * elements, unit inside a head), out [tokens, heads, head_dim] of the same kind, contiguous; lse, f32 [tokens, heads]
+ * or NULL, receives the natural logarithm of the sum of exponentials (-inf for a row that sees no key).
+ * max_new is an upper bound of the new tokens of one sequence (0: unknown); a tight one saves launches.
+ * Scores, statistics and sums are f32; the weights enter the product with V as f16.  Scales below 1e-30 count as
+ * 1e-30. */
+h3q_status h3q_kv_attention(const h3q_kv_cache* cache, const void* q, int kind, int64_t q_token_stride,
+                            int64_t q_head_stride, int64_t tokens, int64_t heads, const int32_t* page_table,
+                            int64_t table_width, const int32_t* lengths, const int32_t* starts, int64_t batch,
+                            int64_t max_new, float scale, int causal, int64_t window, void* out, float* lse,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
