@@ -80,4 +80,7 @@ __device__ __forceinline__ int64_t kv_row_out(const KvAttnArgs& a, const KvSlot&
   return (int64_t)(t.s0 + rr / a.per) * a.heads + kvh * a.per + rr % a.per;
 }
 
+// joins the parts of items that were cut between CTAs, and writes the rows of slots without keys
+cudaError_t launch_kv_attn_join(const KvAttnArgs& a, int tile, cudaStream_t st);
+
 }  // namespace h3q

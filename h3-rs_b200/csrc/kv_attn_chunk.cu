@@ -1,0 +1,695 @@
+// kv_attn_chunk.cu -- attention over the 8-bit paged cache for many query rows to a kv head (prompts, chunks of one,
+// blocks of a stream): bound by the 16-bit tensor cores and the exponentials.
+//
+// A slot is 256 rows of a (sequence, kv head) -- (token, query head of the group) in that order, so a kv head's keys
+// serve all its query heads -- as two 128-row tiles.  512 threads:
+//   warp 0       one lane issues the MMAs: S_t = Q_t K_j^T as soon as softmax t has read S_t, then O_t += W_t V_j
+//                (tcgen05 kind::f16, S and O in TMEM); it also holds the TMEM allocation;
+//   warps 4-11   softmax of tile 0 and 1: thread = row = TMEM lane; scales, maximum, W = 2^(t - m) as f16 into shared
+//                memory, row sums; the maximum moves only when a tile raises it by more than 2^8;
+//   warps 12-15  widen codes to f16 into a ring of three 128-key tiles, in the order the MMAs take them (K0, K1, V0,
+//                K2, V1, ...): codes come straight from global memory into registers one tile ahead, K rows go out as
+//                they are, V is transposed on the way (byte permutes between eight keys of a thread), both in the
+//                K-major 128-byte-swizzle layout.
+// A page's scales never touch the codes (kv_attn.cuh).  Work is cut in 128-key tiles: a first kernel lists the slots
+// that have keys with their running sum, and the CTAs take equal contiguous ranges of the tiles of all (slot, kv head)
+// in order, so no wave is left part full; an item cut between CTAs is joined from f32 parts in order.
+// Every wait is bounded: on time-out the CTA latches an error code, waits for its MMAs, frees TMEM and returns.
+#include <cstdint>
+#include <cuda_runtime.h>
+#include "kv_attn.cuh"
+#include "h3q_internal.h"
+
+namespace h3q {
+
+namespace {
+
+constexpr int BM = 128, BN = 128, NQ = 2, ROWS = NQ * BM;
+constexpr int THREADS = 512;
+constexpr int RING = 3, SC = 4;
+// setmaxnreg split of the 128 registers a thread at launch (512 x 128 = the whole file): MMA 40, softmax 2 x 184,
+// decode 104: 40 + 2 * 184 + 104 = 512 = 4 * 128.
+constexpr int REGS_MMA = 40, REGS_SOFT = 184, REGS_DEC = 104;
+static_assert(REGS_MMA + 2 * REGS_SOFT + REGS_DEC <= 4 * 128, "setmaxnreg split exceeds the launch");
+constexpr uint32_t TMEM_COLS = 512;
+constexpr float kMove = 8.f;
+
+template <int D>
+struct Cfg {
+  static constexpr int Q_SLAB = BM * 128;            // 64 columns of a 128-row tile
+  static constexpr int Q_TILE = (D / 64) * Q_SLAB;
+  static constexpr int KV_TILE = BN * D * 2;         // K: D / 64 slabs of 128 keys; V^T: 2 slabs of 64 keys x D
+  static constexpr int V_SLAB = D * 128;
+  static constexpr int P_SLAB = BM * 128;
+  static constexpr int P_TILE = 2 * P_SLAB;
+  static constexpr int OFF_KV = NQ * Q_TILE;
+  static constexpr int OFF_P = OFF_KV + RING * KV_TILE;
+  static constexpr int OFF_SC = OFF_P + NQ * P_TILE;
+  static constexpr int OFF_BAR = OFF_SC + SC * 8 * 16;
+  static constexpr int NBAR = 2 * RING + SC + 5 * NQ + 1;
+  static constexpr size_t SMEM = 1024 + OFF_BAR + NBAR * 8 + 16;
+  static_assert(SMEM <= 232448, "shared memory exceeds the sm_100 per-CTA limit");
+};
+
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+}  // namespace
+
+// A slot that has keys, and the 128-key tiles of all kv heads before it.
+struct KvListed {
+  int64_t before;
+  int slot, b, tiles, pad;
+};
+struct KvChunkWork {
+  KvListed* list;
+  int64_t* head;  // [0] listed slots, [1] tiles of all
+};
+
+// One CTA: lists the slots with keys in order.
+__global__ void __launch_bounds__(1024) kv_attn_list_kernel(const KvAttnArgs a, const KvChunkWork wk) {
+  __shared__ int sum_n[32], sum_t[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t tiles_before = 0;
+  int64_t count = 0;
+  for (int64_t base = 0; base < a.slots; base += 1024) {
+    const int64_t slot = base + threadIdx.x;
+    int b = 0, tiles = 0;
+    if (slot < a.slots) {
+      b = a.one ? (int)slot : kv_slot_seq(a.s, slot, a.per, ROWS, 1);
+      KvSlot t;
+      if (kv_slot(a, slot, b, ROWS, t)) tiles = (int)((t.hi - t.lo + BN - 1) / BN);
+    }
+    int n = tiles > 0, x = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int n2 = __shfl_up_sync(0xffffffffu, n, o), x2 = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) {
+        n += n2;
+        x += x2;
+      }
+    }
+    if (lane == 31) {
+      sum_n[warp] = n;
+      sum_t[warp] = x;
+    }
+    __syncthreads();
+    int bn = 0, an = 0;
+    int64_t bt = 0, at = 0;
+    for (int w = 0; w < 32; ++w) {
+      if (w < warp) {
+        bn += sum_n[w];
+        bt += sum_t[w];
+      }
+      an += sum_n[w];
+      at += sum_t[w];
+    }
+    if (tiles > 0) {
+      KvListed e;
+      e.before = (tiles_before + bt + x - tiles) * a.c.kv_heads;
+      e.slot = (int)slot;
+      e.b = b;
+      e.tiles = tiles;
+      e.pad = 0;
+      wk.list[count + bn + n - 1] = e;
+    }
+    count += an;
+    tiles_before += at;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    wk.head[0] = count;
+    wk.head[1] = tiles_before * a.c.kv_heads;
+  }
+}
+
+namespace {
+
+// A CTA's walk over its range of tiles: every role steps through the same segments.
+struct Walk {
+  int64_t x, end;
+  int i;  // index into the list
+};
+struct Segment {
+  KvSlot sl;
+  KvListed e;
+  int kvh, t0, t1;  // tiles [t0, t1) of the item
+};
+__device__ __forceinline__ bool next_segment(const KvAttnArgs& a, const KvChunkWork& wk, Walk& w, Segment& s) {
+  if (w.x >= w.end) return false;
+  s.e = wk.list[w.i];
+  if (w.x >= s.e.before + (int64_t)s.e.tiles * a.c.kv_heads) s.e = wk.list[++w.i];
+  const int64_t rel = w.x - s.e.before;
+  s.kvh = (int)(rel / s.e.tiles);
+  s.t0 = (int)(rel - (int64_t)s.kvh * s.e.tiles);
+  s.t1 = (int)(w.end - w.x < s.e.tiles - s.t0 ? s.t0 + (w.end - w.x) : s.e.tiles);
+  kv_slot(a, s.e.slot, s.e.b, ROWS, s.sl);
+  w.x += s.t1 - s.t0;
+  return true;
+}
+
+}  // namespace
+
+template <int D, int CODES>
+__global__ void __launch_bounds__(THREADS, 1)
+    kv_attn_chunk_kernel(const KvAttnArgs a, const KvChunkWork wk, int q_vec, int* err) {
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float4* consts = reinterpret_cast<float4*>(smem + C::OFF_SC);  // [SC][8]: k scale, log2 of the v scale, its inverse
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* kv_empty = kv_full + RING;
+  uint64_t* sc_full = kv_empty + RING;
+  uint64_t* q_full = sc_full + SC;
+  uint64_t* s_full = q_full + NQ;
+  uint64_t* s_free = s_full + NQ;
+  uint64_t* p_full = s_free + NQ;
+  uint64_t* pv_done = p_full + NQ;
+  uint64_t* mma_done = pv_done + NQ;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ int first_i;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t all = wk.head[1], workers = all < gridDim.x ? all : gridDim.x;
+  if (blockIdx.x >= workers) return;
+  Walk walk{all * blockIdx.x / workers, all * (blockIdx.x + 1) / workers, 0};
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < RING; ++i) { mbar_init(&kv_full[i], 4); mbar_init(&kv_empty[i], 1); }
+    for (int i = 0; i < SC; ++i) mbar_init(&sc_full[i], 1);
+    for (int t = 0; t < NQ; ++t) {
+      mbar_init(&q_full[t], 4);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&s_free[t], 4);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&pv_done[t], 1);
+    }
+    mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    int lo = 0, hi = (int)wk.head[0];  // the last listed slot whose tiles begin at or before x
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (wk.list[mid].before <= walk.x) lo = mid;
+      else hi = mid;
+    }
+    first_i = lo;
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  walk.i = first_i;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_MMA));
+    if (warp == 0 && elect_one()) {
+      // ------------------------------------------------------------------ MMA issuer
+      constexpr uint32_t idq = idesc_f16(BM, BN, false);
+      constexpr uint32_t idp = idesc_f16(BM, D, false);
+      const uint32_t q0 = smem_u32(smem), kv0 = smem_u32(smem + C::OFF_KV), p0 = smem_u32(smem + C::OFF_P);
+      uint32_t seq = 0, segs[NQ] = {0, 0}, done[NQ] = {0, 0};  // ring entries, segments and tiles issued
+      bool ok = true;
+      auto wait_kv = [&]() {
+        if (!mbar_wait_bounded(&kv_full[seq % RING], (seq / RING) & 1, abort_flag, err, kDevTimeoutFull)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto issue_qk = [&](int t) {
+        if (done[t] > 0 &&
+            !mbar_wait_bounded(&s_free[t], (done[t] - 1) & 1, abort_flag, err, kDevTimeoutAccEmpty)) return false;
+        tc_fence_after();
+        const uint32_t kb = kv0 + (seq % RING) * C::KV_TILE;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_f16(tmem_base + t * BN, smem_desc_k128(q0 + t * C::Q_TILE + (k >> 2) * C::Q_SLAB) + (uint64_t)(2 * (k & 3)),
+                  smem_desc_k128(kb + (k >> 2) * C::Q_SLAB) + (uint64_t)(2 * (k & 3)), idq, k != 0);
+        mma_commit(&s_full[t]);
+        return true;
+      };
+      Segment s;
+      while (ok && next_segment(a, wk, walk, s)) {
+        const int nq = s.sl.rows > BM ? 2 : 1, n = s.t1 - s.t0;
+        for (int t = 0; ok && t < nq; ++t) {
+          ok = mbar_wait_bounded(&q_full[t], segs[t] & 1, abort_flag, err, kDevTimeoutFull);
+          ++segs[t];
+        }
+        if (!ok || !(ok = wait_kv())) break;
+        for (int t = 0; ok && t < nq; ++t) ok = issue_qk(t);
+        if (!ok) break;
+        mma_commit(&kv_empty[seq % RING]);
+        ++seq;
+        for (int j = 0; ok && j < n; ++j) {
+          if (j + 1 < n) {
+            if (!(ok = wait_kv())) break;
+            for (int t = 0; ok && t < nq; ++t) {
+              ++done[t];
+              ok = issue_qk(t);
+              --done[t];
+            }
+            if (!ok) break;
+            mma_commit(&kv_empty[seq % RING]);
+            ++seq;
+          }
+          if (!(ok = wait_kv())) break;
+          const uint32_t vb = kv0 + (seq % RING) * C::KV_TILE;
+          for (int t = 0; ok && t < nq; ++t) {
+            if (!(ok = mbar_wait_bounded(&p_full[t], done[t] & 1, abort_flag, err, kDevTimeoutProbs))) break;
+            tc_fence_after();
+            const uint32_t pb = p0 + t * C::P_TILE;
+#pragma unroll
+            for (int k = 0; k < BN / 16; ++k)
+              mma_f16(tmem_base + NQ * BN + t * D, smem_desc_k128(pb + (k >> 2) * C::P_SLAB) + (uint64_t)(2 * (k & 3)),
+                      smem_desc_k128(vb + (k >> 2) * C::V_SLAB) + (uint64_t)(2 * (k & 3)), idp, (j | k) != 0);
+            mma_commit(&pv_done[t]);
+            ++done[t];
+          }
+          if (!ok) break;
+          mma_commit(&kv_empty[seq % RING]);
+          ++seq;
+        }
+      }
+      mma_commit(mma_done);  // every MMA issued here completes before TMEM is released
+      mbar_drain(mma_done, 0, err, kDevTimeoutDrain);
+    }
+  } else if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_DEC));
+    // -------------------------------------------------------------------- decode warps
+    const int dw = warp - 12;
+    constexpr int LPR = D / 16;                 // lanes to a K row
+    constexpr int RPP = 128 / LPR;              // K rows of a pass of the four warps: 16 (D = 128) or 32
+    constexpr int KP = BN / RPP;                // passes
+    constexpr int NV = D / 16;                  // words of a V row a thread takes: 4 (16 codes) or 2 ... see vq below
+    const int krow = (dw * 32 + lane) / LPR, kch = lane % LPR;
+    // V: eight keys (octet vo of the tile) and D / 8 columns (chunk vc) a thread
+    const int vo = (lane & 7) + 8 * (dw >> 1), vc = (lane >> 3) + 4 * (dw & 1);
+    constexpr int VW = D / 32;                  // words of a chunk
+    (void)NV;
+    uint4 kbuf[KP];
+    uint32_t vbuf[8][VW];
+    uint32_t seq = 0, tile = 0;
+    bool ok = true;
+    Segment s;
+    while (ok && next_segment(a, wk, walk, s)) {
+      const int n = s.t1 - s.t0;
+      const int64_t key_base = s.sl.lo + (int64_t)s.t0 * BN;
+      // page of the 16 keys at `key`, -1 where the item has none
+      auto page_of = [&](int64_t key) -> int64_t {
+        return key < s.sl.hi ? kv_page(a.c, a.s, s.sl.b, key >> a.c.page_log2) : -1;
+      };
+      auto load_k = [&](int j) {
+        int64_t off[KP];
+#pragma unroll
+        for (int p = 0; p < KP; ++p) {
+          const int64_t key = key_base + (int64_t)j * BN + p * RPP + krow;
+          const int64_t page = page_of(key & ~(int64_t)15);
+          off[p] = page < 0 ? -1 : ((page * a.c.kv_heads + s.kvh) * a.c.page + (key & (a.c.page - 1))) * D + kch * 16;
+        }
+#pragma unroll
+        for (int p = 0; p < KP; ++p)
+          kbuf[p] = off[p] < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(a.c.k + off[p]));
+      };
+      auto load_v = [&](int j) {
+        const int64_t key = key_base + (int64_t)j * BN + vo * 8;
+        const int64_t page = page_of(key & ~(int64_t)15);
+        const int64_t left = s.sl.len - key;  // what lies behind the last token may be any bits
+        const uint8_t* src =
+            a.c.v + (page < 0 ? 0 : ((page * a.c.kv_heads + s.kvh) * a.c.page + (key & (a.c.page - 1))) * D + vc * (D / 8));
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const bool there = page >= 0 && r < left;
+          if (VW == 4) {
+            const uint4 v = there ? __ldg(reinterpret_cast<const uint4*>(src + r * D)) : make_uint4(0, 0, 0, 0);
+            vbuf[r][0] = v.x;
+            vbuf[r][1] = v.y;
+            vbuf[r][VW - 2] = v.z;
+            vbuf[r][VW - 1] = v.w;
+          } else {
+            const uint2 v = there ? __ldg(reinterpret_cast<const uint2*>(src + r * D)) : make_uint2(0, 0);
+            vbuf[r][0] = v.x;
+            vbuf[r][1] = v.y;
+          }
+        }
+      };
+      auto wait_slot = [&]() {
+        return __all_sync(0xffffffffu, mbar_wait_bounded(&kv_empty[seq % RING], ((seq / RING) & 1) ^ 1, abort_flag, err,
+                                                         kDevTimeoutEmpty));
+      };
+      auto publish = [&]() {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kv_full[seq % RING]);
+        ++seq;
+      };
+      auto put_k = [&](int j) {
+        if (!wait_slot()) return false;
+        const uint32_t dst = smem_u32(smem + C::OFF_KV + (seq % RING) * C::KV_TILE);
+#pragma unroll
+        for (int p = 0; p < KP; ++p) {
+          uint32_t h[8];
+          kv_decode4<CODES>(kbuf[p].x, h[0], h[1]);
+          kv_decode4<CODES>(kbuf[p].y, h[2], h[3]);
+          kv_decode4<CODES>(kbuf[p].z, h[4], h[5]);
+          kv_decode4<CODES>(kbuf[p].w, h[6], h[7]);
+          const int row = p * RPP + krow, ch = (kch & 3) * 2;  // 16 columns: two 16-byte chunks of slab kch / 4
+          const uint32_t rb = dst + (kch >> 2) * C::Q_SLAB + row * 128;
+          sts128(rb + ((ch ^ (row & 7)) << 4), h[0], h[1], h[2], h[3]);
+          sts128(rb + (((ch + 1) ^ (row & 7)) << 4), h[4], h[5], h[6], h[7]);
+        }
+        if (dw == 0) {  // the scales of the tile's eight 16-key groups
+          if (lane < 8) {
+            const int64_t page = page_of(key_base + (int64_t)j * BN + lane * 16);
+            float4 c = make_float4(0.f, -INFINITY, 0.f, 0.f);
+            if (page >= 0) {
+              const float vs = fmaxf(__ldg(a.c.v_scale + page * a.c.kv_heads + s.kvh), kKvScaleFloor);
+              c = make_float4(__ldg(a.c.k_scale + page * a.c.kv_heads + s.kvh), kv_lg2(vs), __fdividef(1.f, vs), 0.f);
+            }
+            consts[(tile % SC) * 8 + lane] = c;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sc_full[tile % SC]);
+        }
+        ++tile;
+        publish();
+        return true;
+      };
+      auto put_v = [&]() {
+        if (!wait_slot()) return false;
+        const uint32_t dst = smem_u32(smem + C::OFF_KV + (seq % RING) * C::KV_TILE) + (vo >> 3) * C::V_SLAB;
+#pragma unroll
+        for (int q = 0; q < VW; ++q) {
+          uint32_t h[4][4];  // [column][key pair]
+#pragma unroll
+          for (int kp = 0; kp < 4; ++kp) {
+            kv_decode4<CODES>(prmt(vbuf[2 * kp][q], vbuf[2 * kp + 1][q], 0x5140), h[0][kp], h[1][kp]);
+            kv_decode4<CODES>(prmt(vbuf[2 * kp][q], vbuf[2 * kp + 1][q], 0x7362), h[2][kp], h[3][kp]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int d = vc * (D / 8) + q * 4 + e;
+            sts128(dst + d * 128 + (((vo & 7) ^ (d & 7)) << 4), h[e][0], h[e][1], h[e][2], h[e][3]);
+          }
+        }
+        publish();
+        return true;
+      };
+      load_k(0);
+      ok = put_k(0);
+      if (!ok) break;
+      if (n > 1) load_k(1);
+      load_v(0);
+      for (int j = 0; ok && j < n; ++j) {
+        if (j + 1 < n) {
+          ok = put_k(j + 1);
+          if (!ok) break;
+          if (j + 2 < n) load_k(j + 2);
+        }
+        ok = put_v();
+        if (ok && j + 1 < n) load_v(j + 1);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFT));
+    // -------------------------------------------------------------------- softmax warps
+    const int g = (warp - 4) >> 2;
+    const int quarter = warp & 3;
+    const int rloc = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tS = tmem_base + lane_off + g * BN;
+    const uint32_t tO = tmem_base + lane_off + NQ * BN + g * D;
+    const uint32_t prow = smem_u32(smem + C::OFF_P + g * C::P_TILE) + rloc * 128;
+    const uint32_t qrow = smem_u32(smem + g * C::Q_TILE) + rloc * 128;
+    const uint32_t swz = rloc & 7;
+    uint32_t done = 0, tile0 = 0;
+    bool ok = true, first = true;
+    Segment s;
+    while (ok && next_segment(a, wk, walk, s)) {
+      const int n = s.t1 - s.t0;
+      const bool whole = s.t0 == 0 && s.t1 == s.e.tiles;
+      const int part_slot = (int)blockIdx.x * 2 + (first ? 0 : 1);
+      first = false;
+      if (s.t0 == 0 && g == 0 && rloc == 0) {
+        const int64_t y = s.e.before + (int64_t)(s.kvh + 1) * s.e.tiles - 1;
+        const int64_t w1 = ((y + 1) * workers - 1) / all;
+        a.meta[(int64_t)s.e.slot * a.c.kv_heads + s.kvh] = make_int4(part_slot, (int)(w1 - blockIdx.x) + 1, (int)blockIdx.x, 0);
+      }
+      if (g * BM >= s.sl.rows) {  // a slot of one tile
+        tile0 += n;
+        continue;
+      }
+      const int r = g * BM + rloc;
+      const bool in = r < s.sl.rows;
+      // ------------------------------------------------------------ q as f16, the sign of the scale in it
+      float c = fabsf(a.scale_log2);
+      {
+        const int rr = s.sl.r0 + (in ? r : 0);
+        const uint16_t* src =
+            a.q + (int64_t)(s.sl.s0 + rr / a.per) * a.q_ts + (int64_t)(s.kvh * a.per + rr % a.per) * a.q_hs;
+        uint32_t w[D / 2];
+        if (q_vec) {
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const uint4 v = in ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+            w[4 * i] = v.x;
+            w[4 * i + 1] = v.y;
+            w[4 * i + 2] = v.z;
+            w[4 * i + 3] = v.w;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < D / 2; ++i)
+            w[i] = in ? (uint32_t)__ldg(src + 2 * i) | ((uint32_t)__ldg(src + 2 * i + 1) << 16) : 0u;
+        }
+        if (a.kind == 2) {
+          float mx = 0.f;
+#pragma unroll
+          for (int i = 0; i < D / 2; ++i)
+            mx = max3f(mx, fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u)));
+          float f = 1.f;
+          if (mx > 0.f && mx < INFINITY) {
+            const int e = ilogbf(mx);
+            // 2^-e in two factors: e reaches 127 and (for bf16 below the normal range) -133
+            f = scalbnf(1.f, -e / 2);
+            c = scalbnf(c, e);
+            const float f2nd = scalbnf(1.f, -e - (-e / 2));
+#pragma unroll
+            for (int i = 0; i < D / 2; ++i)
+              w[i] = kv_pack_f16(__uint_as_float(w[i] << 16) * f * f2nd, __uint_as_float(w[i] & 0xffff0000u) * f * f2nd);
+          } else {
+#pragma unroll
+            for (int i = 0; i < D / 2; ++i)
+              w[i] = kv_pack_f16(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+          }
+        }
+        const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+        // the last segment's S of this tile is read, so its MMAs are done with Q
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+          sts128(qrow + (i >> 3) * C::Q_SLAB + (((i & 7) ^ swz) << 4), w[4 * i] ^ sign, w[4 * i + 1] ^ sign,
+                 w[4 * i + 2] ^ sign, w[4 * i + 3] ^ sign);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[g]);
+      }
+      const int64_t key_base = s.sl.lo + (int64_t)s.t0 * BN;
+      int64_t lo = 0, hi = 0;
+      if (in) kv_row_keys(a, s.sl, r, lo, hi);
+      lo -= key_base;
+      hi -= key_base;
+      float m_used = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&s_full[g], done & 1, abort_flag, err, kDevTimeoutScores))) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t sr[BN / 32][32];
+#pragma unroll
+        for (int k = 0; k < BN / 32; ++k) tmem_ld_32x32b_x32(tS + 32 * k, sr[k]);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[g]);
+        const uint32_t T = tile0 + j;
+        if (!__all_sync(0xffffffffu,
+                        mbar_wait_bounded(&sc_full[T % SC], (T / SC) & 1, abort_flag, err, kDevTimeoutScale))) {
+          ok = false;
+          break;
+        }
+        const float4* cs = consts + (T % SC) * 8;
+        const int64_t k0 = (int64_t)j * BN;
+        if (__any_sync(0xffffffffu, lo > k0 || hi < k0 + BN)) {  // some row does not see the whole tile
+          const int a0 = (int)(lo - k0 < 0 ? 0 : (lo - k0 > BN ? BN : lo - k0));
+          const int a1 = (int)(hi - k0 < 0 ? 0 : (hi - k0 > BN ? BN : hi - k0));
+#pragma unroll
+          for (int i = 0; i < BN; ++i)
+            if (i < a0 || i >= a1) sr[i >> 5][i & 31] = 0xff800000u;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          float mg[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            mg[i & 1] = max3f(mg[i & 1], __uint_as_float(sr[q >> 1][(q & 1) * 16 + 2 * i]),
+                              __uint_as_float(sr[q >> 1][(q & 1) * 16 + 2 * i + 1]));
+          const float4 cq = cs[q];
+          // at least 1e-37, so that a masked -inf stays -inf for a scale of 0
+          mx = fmaxf(mx, __fmaf_rn(fmaxf(mg[0], mg[1]), fmaxf(c * cq.x, 1e-37f), cq.y));
+        }
+        const bool move = mx > m_used + kMove;
+        float alpha = 1.f;
+        if (move) {
+          alpha = kv_ex2(m_used - mx);
+          m_used = mx;
+        }
+        l *= alpha;
+        const float m = m_used == -INFINITY ? 0.f : m_used;
+        uint32_t pk16[BN / 2];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float4 cq = cs[q];
+          const float ck = fmaxf(c * cq.x, 1e-37f), off = cq.y - m;
+          const f2 c2 = pk(ck, ck), o2 = pk(off, off);
+          f2 la = pk(0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float t0, t1;
+            upk(fma2(pk(__uint_as_float(sr[q >> 1][(q & 1) * 16 + 2 * i]),
+                        __uint_as_float(sr[q >> 1][(q & 1) * 16 + 2 * i + 1])),
+                     c2, o2),
+                t0, t1);
+            const float p0 = kv_ex2(t0), p1 = kv_ex2(t1);
+            la = add2(la, pk(p0, p1));
+            pk16[q * 8 + i] = kv_pack_f16(p0, p1);
+          }
+          float s0, s1;
+          upk(la, s0, s1);
+          l = __fmaf_rn(s0 + s1, cq.z, l);
+        }
+        // W_g and O_g are free once the previous tile's product has completed
+        if (j > 0) {
+          if (!__all_sync(0xffffffffu,
+                          mbar_wait_bounded(&pv_done[g], (done - 1) & 1, abort_flag, err, kDevTimeoutPV))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+            for (int k = 0; k < D / 32; ++k) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(tO + 32 * k, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x32b_x32(tO + 32 * k, o);
+            }
+            tmem_wait_st();
+          }
+        }
+#pragma unroll
+        for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t* q4 = &pk16[sl * 32 + k * 4];
+            sts128(prow + sl * C::P_SLAB + ((k ^ swz) << 4), q4[0], q4[1], q4[2], q4[3]);
+          }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[g]);
+        ++done;
+      }
+      if (!ok) break;
+      tile0 += n;
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&pv_done[g], (done - 1) & 1, abort_flag, err, kDevTimeoutPV))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int64_t ro = in ? kv_row_out(a, s.sl, s.kvh, r) : 0;
+      float* part = a.part + (int64_t)part_slot * ROWS * (D + 2);
+      const float inv = l > 0.f ? __fdiv_rn(1.f, l) : (l == 0.f ? 0.f : l);  // a NaN goes through
+#pragma unroll 1
+      for (int k = 0; k < D / 32; ++k) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(tO + 32 * k, o);
+        tmem_wait_ld();
+        if (!in) continue;
+        if (whole) {
+          uint4* d4 = reinterpret_cast<uint4*>(a.out + ro * D + 32 * k);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = kv_pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv, a.kind);
+            d4[i] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else {
+          uint4* d4 = reinterpret_cast<uint4*>(part + (int64_t)r * D + 32 * k);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d4[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+      }
+      if (in) {
+        if (!whole) *reinterpret_cast<float2*>(part + (int64_t)ROWS * D + 2 * r) = make_float2(m_used, l);
+        else if (a.lse) a.lse[ro] = l == 0.f ? -INFINITY : 0.6931471805599453f * (m_used + log2f(l));
+      }
+      tc_fence_before();  // the reads of O are ordered before the next segment's first product, through p_full
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+namespace {
+
+template <int D, int CODES>
+cudaError_t launch_chunk(const KvAttnArgs& a, const KvChunkWork& wk, int q_vec, int* err, cudaStream_t st) {
+  auto kern = kv_attn_chunk_kernel<D, CODES>;
+  static bool ready[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!ready[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<D>::SMEM);
+    if (e != cudaSuccess) return e;
+    ready[dev] = true;
+  }
+  kv_attn_list_kernel<<<1, 1024, 0, st>>>(a, wk);
+  if (const cudaError_t e = cudaGetLastError()) return e;
+  kern<<<(unsigned)sm_count(dev), THREADS, Cfg<D>::SMEM, st>>>(a, wk, q_vec, err);
+  if (const cudaError_t e = cudaGetLastError()) return e;
+  return launch_kv_attn_join(a, ROWS, st);
+}
+
+}  // namespace
+
+size_t kv_attn_chunk_part_bytes(int dim) { return (size_t)sm_count(0) * 2 * ROWS * (dim + 2) * 4; }
+size_t kv_attn_chunk_list_bytes(int64_t slots) { return 256 + (size_t)slots * sizeof(KvListed); }
+
+cudaError_t launch_kv_attn_chunk(const KvAttnArgs& a, void* list, int* err, cudaStream_t st) {
+  KvChunkWork wk;
+  wk.head = static_cast<int64_t*>(list);
+  wk.list = reinterpret_cast<KvListed*>(static_cast<uint8_t*>(list) + 256);
+  const int q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15u) == 0 && a.q_ts % 8 == 0 && a.q_hs % 8 == 0;
+#define H3Q_KV_C(DD, CC) \
+  if (a.c.dim == DD && a.c.codes == CC) return launch_chunk<DD, CC>(a, wk, q_vec, err, st);
+  H3Q_KV_C(64, 0) H3Q_KV_C(64, 1) H3Q_KV_C(128, 0) H3Q_KV_C(128, 1)
+#undef H3Q_KV_C
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace h3q

@@ -491,10 +491,12 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
   }
 }
 
+}  // namespace
+
 // Joins the parts of the items that were cut, in their order, and writes the rows of slots without keys: a warp a row.
-template <int D, int MT>
+template <int D, int TILE>
 __global__ void __launch_bounds__(256) kv_attn_join_kernel(const KvAttnArgs a) {
-  constexpr int TILE = MT * 16, E = D / 32;
+  constexpr int E = D / 32;
   const int64_t item = blockIdx.x;
   const int64_t slot = item / a.c.kv_heads;
   const int kvh = (int)(item % a.c.kv_heads);
@@ -532,6 +534,20 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(const KvAttnArgs a) {
   }
 }
 
+cudaError_t launch_kv_attn_join(const KvAttnArgs& a, int tile, cudaStream_t st) {
+  const unsigned grid = (unsigned)(a.slots * a.c.kv_heads);
+#define H3Q_KV_J(DD, TT)                                     \
+  if (a.c.dim == DD && tile == TT) {                         \
+    kv_attn_join_kernel<DD, TT><<<grid, 256, 0, st>>>(a);    \
+    return cudaGetLastError();                               \
+  }
+  H3Q_KV_J(64, 16) H3Q_KV_J(64, 32) H3Q_KV_J(64, 256) H3Q_KV_J(128, 16) H3Q_KV_J(128, 32) H3Q_KV_J(128, 256)
+#undef H3Q_KV_J
+  return cudaErrorInvalidValue;
+}
+
+namespace {
+
 template <int D, int CODES, int MT>
 cudaError_t launch_rows(KvAttnArgs a, cudaStream_t st) {
   using C = RowsCfg<D, MT>;
@@ -547,8 +563,7 @@ cudaError_t launch_rows(KvAttnArgs a, cudaStream_t st) {
   }
   kern<<<(unsigned)(sm_count(dev) * (MT == 1 ? 2 : 1)), kThreads, C::kSmem, st>>>(a);
   if (const cudaError_t e = cudaGetLastError()) return e;
-  kv_attn_join_kernel<D, MT><<<(unsigned)(a.slots * a.c.kv_heads), 256, 0, st>>>(a);
-  return cudaGetLastError();
+  return launch_kv_attn_join(a, MT * 16, st);
 }
 
 }  // namespace

@@ -18,6 +18,9 @@ cudaError_t launch_kv_read(const KvCache& c, const KvSeqs& s, const int32_t* fir
                            cudaStream_t st);
 size_t kv_attn_rows_part_bytes(int dim, int tile);
 cudaError_t launch_kv_attn_rows(const KvAttnArgs& a, int tile, cudaStream_t st);
+size_t kv_attn_chunk_part_bytes(int dim);
+size_t kv_attn_chunk_list_bytes(int64_t slots);
+cudaError_t launch_kv_attn_chunk(const KvAttnArgs& a, void* list, int* err, cudaStream_t st);
 }  // namespace h3q
 
 using namespace h3q;
@@ -103,24 +106,34 @@ KvSeqs seqs_of(const int32_t* table, int64_t width, const int32_t* starts, int64
   return s;
 }
 
-// How a call's attention is cut: the row kernel takes the sequences of up to `rows` query rows to a kv head.
+// How a call's attention is cut: the row kernel takes the sequences of up to 32 query rows (new tokens times the query
+// heads of a kv head), the chunk kernel the others.  Each has its own part of the workspace.
 struct AttnPlan {
-  int tile;        // rows of a slot of the row kernel
-  int one;         // every sequence has one slot
-  int64_t slots;
-  size_t part, meta, bytes;
+  int tile;        // rows of a slot of the row kernel, 0: none of the sequences can be its
+  int chunk;       // the chunk kernel runs
+  int64_t slots, chunk_slots;
+  size_t part, meta, chunk_part, chunk_meta, chunk_list, bytes;
 };
 
-AttnPlan plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t max_new, int dim) {
+constexpr int kRowsMax = 32;
+
+AttnPlan plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int64_t max_new, bool even, int dim) {
   AttnPlan p{};
-  const int64_t per = heads / kv_heads;
-  const int64_t most = max_new * per;
-  p.tile = most <= 16 ? 16 : 32;
-  p.one = most <= p.tile;
-  p.slots = p.one ? batch : tokens * per / p.tile + batch;
-  p.part = a256(kv_attn_rows_part_bytes(dim, p.tile));
-  p.meta = a256((size_t)p.slots * (size_t)kv_heads * sizeof(int4));
-  p.bytes = p.part + p.meta;
+  const int64_t per = heads / kv_heads, most = max_new * per;
+  p.chunk = most > kRowsMax;
+  p.tile = p.chunk && even ? 0 : (most <= 16 ? 16 : kRowsMax);
+  if (p.tile) {
+    p.slots = batch;
+    p.part = a256(kv_attn_rows_part_bytes(dim, p.tile));
+    p.meta = a256((size_t)p.slots * (size_t)kv_heads * sizeof(int4));
+  }
+  if (p.chunk) {
+    p.chunk_slots = tokens * per / 256 + batch;
+    p.chunk_part = a256(kv_attn_chunk_part_bytes(dim));
+    p.chunk_meta = a256((size_t)p.chunk_slots * (size_t)kv_heads * sizeof(int4));
+    p.chunk_list = a256(kv_attn_chunk_list_bytes(p.chunk_slots));
+  }
+  p.bytes = p.part + p.meta + p.chunk_part + p.chunk_meta + p.chunk_list;
   return p;
 }
 
@@ -182,7 +195,8 @@ h3q_status h3q_kv_read(const h3q_kv_cache* cache, const int32_t* page_table, int
 size_t h3q_kv_attention_workspace_size(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, int head_dim,
                                        int64_t max_new) {
   if (tokens <= 0 || batch <= 0 || heads <= 0 || kv_heads <= 0 || max_new < 0) return 0;
-  return plan(tokens, batch, heads, kv_heads, max_new == 0 || max_new > tokens ? tokens : max_new, head_dim).bytes;
+  const int64_t most = max_new == 0 || max_new > tokens ? tokens : max_new;
+  return plan(tokens, batch, heads, kv_heads, most, false, head_dim).bytes;
 }
 
 h3q_status h3q_kv_attention(const h3q_kv_cache* cache, const void* q, int kind, int64_t q_token_stride,
@@ -206,7 +220,7 @@ h3q_status h3q_kv_attention(const h3q_kv_cache* cache, const void* q, int kind, 
   const int64_t most = max_new_of(max_new, starts, batch, tokens);
   if (most * (heads / cache->kv_heads) > (int64_t)1 << 30)
     return fail(H3Q_ERR_UNSUPPORTED, "%s: this build handles 2^30 query rows to a sequence and kv head", what);
-  const AttnPlan p = plan(tokens, batch, heads, cache->kv_heads, most, cache->head_dim);
+  const AttnPlan p = plan(tokens, batch, heads, cache->kv_heads, most, !starts, cache->head_dim);
   const size_t need = h3q_kv_attention_workspace_size(tokens, batch, heads, cache->kv_heads, cache->head_dim,
                                                       starts ? max_new : most);
   if (!workspace || workspace_bytes < need)
@@ -227,14 +241,29 @@ h3q_status h3q_kv_attention(const h3q_kv_cache* cache, const void* q, int kind, 
   a.scale_log2 = scale * 1.44269504088896340736f;
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
-  a.row_lo = 0;
-  a.row_hi = 0x7fffffff;
-  a.one = p.one;
-  a.slots = p.slots;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (p.chunk) {
+    int* err = error_word_current();
+    if (!err) return fail(H3Q_ERR_CUDA, "%s: could not set up the device error word", what);
+    KvAttnArgs b = a;
+    b.row_lo = p.tile;
+    b.row_hi = 0x7fffffff;
+    b.one = 0;
+    b.slots = p.chunk_slots;
+    b.part = reinterpret_cast<float*>(ws);
+    b.meta = reinterpret_cast<int4*>(ws + p.chunk_part);
+    if (h3q_status s = cuda_status(launch_kv_attn_chunk(b, ws + p.chunk_part + p.chunk_meta, err, st), what)) return s;
+    ws += p.chunk_part + p.chunk_meta + p.chunk_list;
+  }
+  if (!p.tile) return H3Q_OK;
+  a.row_lo = 0;
+  a.row_hi = p.tile;
+  a.one = 1;
+  a.slots = p.slots;
   a.part = reinterpret_cast<float*>(ws);
   a.meta = reinterpret_cast<int4*>(ws + p.part);
-  return cuda_status(launch_kv_attn_rows(a, p.tile, static_cast<cudaStream_t>(stream)), what);
+  return cuda_status(launch_kv_attn_rows(a, p.tile, st), what);
 }
 
 }  // extern "C"
