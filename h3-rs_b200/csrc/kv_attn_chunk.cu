@@ -3,12 +3,15 @@
 //
 // A slot is 256 rows of a (sequence, kv head) -- (token, query head of the group) in that order, so a kv head's keys
 // serve all its query heads -- as two 128-row tiles.  512 threads:
-//   warp 0       one lane issues the MMAs: S_t = Q_t K_j^T as soon as softmax t has read S_t, then O_t += W_t V_j
-//                (tcgen05 kind::f16, S and O in TMEM); it also holds the TMEM allocation;
-//   warps 4-11   softmax of tile 0 and 1: thread = row = TMEM lane; scales, maximum, W = 2^(t - m) as f16 into shared
-//                memory, row sums; the maximum moves only when a tile raises it by more than 2^8;
-//   warps 12-15  widen codes to f16 into a ring of three 128-key tiles, in the order the MMAs take them (K0, K1, V0,
-//                K2, V1, ...): codes come straight from global memory into registers one tile ahead, K rows go out as
+//   warp 0       one lane issues the MMAs (tcgen05 kind::f16): per tile pair O_t += W_t V_j and then S_t = Q_t K_(j+1)^T,
+//                t = 0, 1, so that one softmax works while the other's products run; it also holds the TMEM allocation;
+//   warps 4-11   softmax of tile 0 and 1: thread = row = TMEM lane; scales, maximum, W = 2^(t - m) as f16 back into TMEM
+//                over the scores it came from (the A operand of the second product is read from there: with W in
+//                shared memory the products alone would take the SM's whole shared-memory bandwidth), row sums; the
+//                maximum moves only when a tile raises it by more than 2^8;
+//   warp 1       walks the page table ahead of them: the address and the scales of each 16 keys, into a ring in shared
+//                memory, so that the others never wait for a table entry before they can ask for what it names;
+//   warps 12-15  widen codes to f16 into a ring of five 128-key tiles, K and V in turn: codes come straight from global memory into registers one tile ahead, K rows go out as
 //                they are, V is transposed on the way (byte permutes between eight keys of a thread), both in the
 //                K-major 128-byte-swizzle layout.
 // A page's scales never touch the codes (kv_attn.cuh).  Work is cut in 128-key tiles: a first kernel lists the slots
@@ -26,10 +29,10 @@ namespace {
 
 constexpr int BM = 128, BN = 128, NQ = 2, ROWS = NQ * BM;
 constexpr int THREADS = 512;
-constexpr int RING = 3, SC = 4;
-// setmaxnreg split of the 128 registers a thread at launch (512 x 128 = the whole file): MMA 40, softmax 2 x 184,
-// decode 104: 40 + 2 * 184 + 104 = 512 = 4 * 128.
-constexpr int REGS_MMA = 40, REGS_SOFT = 184, REGS_DEC = 104;
+constexpr int RING = 5, WR = 8;
+// setmaxnreg split of the 128 registers a thread at launch (512 x 128 = the whole file): MMA 48, softmax 2 x 184,
+// decode 96: 48 + 2 * 184 + 96 = 512 = 4 * 128.
+constexpr int REGS_MMA = 48, REGS_SOFT = 184, REGS_DEC = 96;
 static_assert(REGS_MMA + 2 * REGS_SOFT + REGS_DEC <= 4 * 128, "setmaxnreg split exceeds the launch");
 constexpr uint32_t TMEM_COLS = 512;
 constexpr float kMove = 8.f;
@@ -40,22 +43,46 @@ struct Cfg {
   static constexpr int Q_TILE = (D / 64) * Q_SLAB;
   static constexpr int KV_TILE = BN * D * 2;         // K: D / 64 slabs of 128 keys; V^T: 2 slabs of 64 keys x D
   static constexpr int V_SLAB = D * 128;
-  static constexpr int P_SLAB = BM * 128;
-  static constexpr int P_TILE = 2 * P_SLAB;
   static constexpr int OFF_KV = NQ * Q_TILE;
-  static constexpr int OFF_P = OFF_KV + RING * KV_TILE;
-  static constexpr int OFF_SC = OFF_P + NQ * P_TILE;
-  static constexpr int OFF_BAR = OFF_SC + SC * 8 * 16;
-  static constexpr int NBAR = 2 * RING + SC + 5 * NQ + 1;
+  static constexpr int OFF_SC = OFF_KV + RING * KV_TILE;
+  static constexpr int OFF_ADDR = OFF_SC + WR * 8 * 16;
+  static constexpr int OFF_BAR = OFF_ADDR + WR * 8 * 8;
+  static constexpr int NBAR = 2 * RING + 2 * WR + 4 * NQ + 1;
   static constexpr size_t SMEM = 1024 + OFF_BAR + NBAR * 8 + 16;
-  static_assert(SMEM <= 232448, "shared memory exceeds the sm_100 per-CTA limit");
+  static_assert(SMEM + 16 <= 232448, "shared memory exceeds the sm_100 per-CTA limit");
 };
+
+// the K-major 128-byte-swizzle descriptor of shared memory at 16 * `lo` bytes
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
+  constexpr uint32_t hi = (1024 >> 4) | (1u << 14) | (2u << 29);  // 8-row stride, version, swizzle
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo | (1u << 16)), "n"(hi));
+  return d;
+}
 
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
 }  // namespace
+
+// x, as a value that the compiler cannot compute ahead of a loop and keep: what is derived from it costs an add where it
+// is used, not a register (or a spill) for the whole kernel
+__device__ __forceinline__ uint32_t fresh(uint32_t x) {
+  asm volatile("" : "+r"(x));
+  return x;
+}
+
+// the values of a TMEM load, used only after the wait before this point
+__device__ __forceinline__ void pin(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+
+template <int V>
+struct Int {
+  static constexpr int value = V;
+};
 
 // A slot that has keys, and the 128-key tiles of all kv heads before it.
 struct KvListed {
@@ -157,16 +184,17 @@ __global__ void __launch_bounds__(THREADS, 1)
   using C = Cfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float4* consts = reinterpret_cast<float4*>(smem + C::OFF_SC);  // [SC][8]: k scale, log2 of the v scale, its inverse
+  float4* consts = reinterpret_cast<float4*>(smem + C::OFF_SC);  // [WR][8]: k scale, log2 of the v scale, its inverse
+  int64_t* addr = reinterpret_cast<int64_t*>(smem + C::OFF_ADDR);  // [WR][8]: offset of the codes of 16 keys, or -1
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* kv_empty = kv_full + RING;
-  uint64_t* sc_full = kv_empty + RING;
-  uint64_t* q_full = sc_full + SC;
+  uint64_t* wr_full = kv_empty + RING;
+  uint64_t* wr_free = wr_full + WR;
+  uint64_t* q_full = wr_free + WR;
   uint64_t* s_full = q_full + NQ;
-  uint64_t* s_free = s_full + NQ;
-  uint64_t* p_full = s_free + NQ;
-  uint64_t* pv_done = p_full + NQ;
-  uint64_t* mma_done = pv_done + NQ;
+  uint64_t* p_full = s_full + NQ;
+  uint64_t* o_full = p_full + NQ;
+  uint64_t* mma_done = o_full + NQ;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ int first_i;
@@ -177,13 +205,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   Walk walk{all * blockIdx.x / workers, all * (blockIdx.x + 1) / workers, 0};
   if (threadIdx.x == 0) {
     for (int i = 0; i < RING; ++i) { mbar_init(&kv_full[i], 4); mbar_init(&kv_empty[i], 1); }
-    for (int i = 0; i < SC; ++i) mbar_init(&sc_full[i], 1);
+    for (int i = 0; i < WR; ++i) { mbar_init(&wr_full[i], 1); mbar_init(&wr_free[i], 4); }
     for (int t = 0; t < NQ; ++t) {
       mbar_init(&q_full[t], 4);
       mbar_init(&s_full[t], 1);
-      mbar_init(&s_free[t], 4);
       mbar_init(&p_full[t], 4);
-      mbar_init(&pv_done[t], 1);
+      mbar_init(&o_full[t], 1);
     }
     mbar_init(mma_done, 1);
     *abort_flag = 0;
@@ -212,70 +239,120 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ------------------------------------------------------------------ MMA issuer
       constexpr uint32_t idq = idesc_f16(BM, BN, false);
       constexpr uint32_t idp = idesc_f16(BM, D, false);
-      const uint32_t q0 = smem_u32(smem), kv0 = smem_u32(smem + C::OFF_KV), p0 = smem_u32(smem + C::OFF_P);
-      uint32_t seq = 0, segs[NQ] = {0, 0}, done[NQ] = {0, 0};  // ring entries, segments and tiles issued
+      // shared-memory addresses in units of 16 bytes: a step in K of 16 columns is 2, of 64 a slab
+      // shared-memory addresses in units of 16 bytes: a step in K of 16 columns is 2, of 64 a slab
+      const uint32_t q0 = smem_u32(smem) >> 4, kv0 = smem_u32(smem + C::OFF_KV) >> 4;
+      uint32_t slot = 0, phase = 0;  // place in the ring
+      uint32_t segs0 = 0, segs1 = 0, done0 = 0, done1 = 0;  // segments and tiles of each row tile
       bool ok = true;
+      auto advance = [&]() {
+        if (++slot == RING) {
+          slot = 0;
+          phase ^= 1;
+        }
+      };
       auto wait_kv = [&]() {
-        if (!mbar_wait_bounded(&kv_full[seq % RING], (seq / RING) & 1, abort_flag, err, kDevTimeoutFull)) return false;
+        if (!mbar_wait_prompt(&kv_full[slot], phase, abort_flag, err, kDevTimeoutFull)) return false;
         tc_fence_after();
         return true;
       };
-      auto issue_qk = [&](int t) {
-        if (done[t] > 0 &&
-            !mbar_wait_bounded(&s_free[t], (done[t] - 1) & 1, abort_flag, err, kDevTimeoutAccEmpty)) return false;
-        tc_fence_after();
-        const uint32_t kb = kv0 + (seq % RING) * C::KV_TILE;
+      // S_t = Q_t K^T
+      auto issue_qk = [&](auto tc) {
+        constexpr int t = decltype(tc)::value;
+        const uint32_t qb = fresh(q0 + t * (C::Q_TILE >> 4)), kb = fresh(kv0 + slot * (C::KV_TILE >> 4));
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          mma_f16(tmem_base + t * BN, smem_desc_k128(q0 + t * C::Q_TILE + (k >> 2) * C::Q_SLAB) + (uint64_t)(2 * (k & 3)),
-                  smem_desc_k128(kb + (k >> 2) * C::Q_SLAB) + (uint64_t)(2 * (k & 3)), idq, k != 0);
-        mma_commit(&s_full[t]);
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t o = (k >> 2) * (C::Q_SLAB >> 4) + 2 * (k & 3);
+          mma_f16(tmem_base + t * BN, desc_of(qb + o), desc_of(kb + o), idq, k != 0);
+        }
+        mma_commit(&s_full[t]);  // completes with every MMA before it, so O_t is also up to date then
+      };
+      // O_t += W_t V, W_t over the first 64 columns of S_t
+      auto issue_pv = [&](auto tc, uint32_t vslot, uint32_t tiles, bool add) {
+        constexpr int t = decltype(tc)::value;
+        if (!mbar_wait_prompt(&p_full[t], tiles & 1, abort_flag, err, kDevTimeoutProbs)) return false;
+        tc_fence_after();
+        const uint32_t vb = fresh(kv0 + vslot * (C::KV_TILE >> 4));
+#pragma unroll
+        for (int k = 0; k < BN / 16; ++k)
+          mma_f16_ts(tmem_base + NQ * BN + t * D, tmem_base + t * BN + 8 * k,
+                     desc_of(vb + (k >> 2) * (C::V_SLAB >> 4) + 2 * (k & 3)), idp, add || k != 0);
         return true;
       };
+      constexpr Int<0> t0{};
+      constexpr Int<1> t1{};
       Segment s;
       while (ok && next_segment(a, wk, walk, s)) {
-        const int nq = s.sl.rows > BM ? 2 : 1, n = s.t1 - s.t0;
-        for (int t = 0; ok && t < nq; ++t) {
-          ok = mbar_wait_bounded(&q_full[t], segs[t] & 1, abort_flag, err, kDevTimeoutFull);
-          ++segs[t];
+        const bool two = s.sl.rows > BM;
+        const int n = s.t1 - s.t0;
+        if (!(ok = wait_kv() && mbar_wait_prompt(&q_full[0], segs0++ & 1, abort_flag, err, kDevTimeoutFull))) break;
+        tc_fence_after();
+        issue_qk(t0);
+        if (two) {
+          if (!(ok = mbar_wait_prompt(&q_full[1], segs1++ & 1, abort_flag, err, kDevTimeoutFull))) break;
+          tc_fence_after();
+          issue_qk(t1);
         }
-        if (!ok || !(ok = wait_kv())) break;
-        for (int t = 0; ok && t < nq; ++t) ok = issue_qk(t);
-        if (!ok) break;
-        mma_commit(&kv_empty[seq % RING]);
-        ++seq;
-        for (int j = 0; ok && j < n; ++j) {
-          if (j + 1 < n) {
-            if (!(ok = wait_kv())) break;
-            for (int t = 0; ok && t < nq; ++t) {
-              ++done[t];
-              ok = issue_qk(t);
-              --done[t];
-            }
-            if (!ok) break;
-            mma_commit(&kv_empty[seq % RING]);
-            ++seq;
-          }
+        mma_commit(&kv_empty[slot]);
+        advance();
+        for (int j = 0; j < n; ++j) {
+          const bool more = j + 1 < n;
+          const uint32_t vslot = slot;
           if (!(ok = wait_kv())) break;
-          const uint32_t vb = kv0 + (seq % RING) * C::KV_TILE;
-          for (int t = 0; ok && t < nq; ++t) {
-            if (!(ok = mbar_wait_bounded(&p_full[t], done[t] & 1, abort_flag, err, kDevTimeoutProbs))) break;
-            tc_fence_after();
-            const uint32_t pb = p0 + t * C::P_TILE;
-#pragma unroll
-            for (int k = 0; k < BN / 16; ++k)
-              mma_f16(tmem_base + NQ * BN + t * D, smem_desc_k128(pb + (k >> 2) * C::P_SLAB) + (uint64_t)(2 * (k & 3)),
-                      smem_desc_k128(vb + (k >> 2) * C::V_SLAB) + (uint64_t)(2 * (k & 3)), idp, (j | k) != 0);
-            mma_commit(&pv_done[t]);
-            ++done[t];
+          advance();
+          if (!(ok = issue_pv(t0, vslot, done0, j > 0) && (!more || wait_kv()))) break;
+          if (more) issue_qk(t0);
+          else mma_commit(&o_full[0]);
+          ++done0;
+          if (two) {
+            if (!(ok = issue_pv(t1, vslot, done1, j > 0))) break;
+            if (more) issue_qk(t1);
+            else mma_commit(&o_full[1]);
+            ++done1;
           }
-          if (!ok) break;
-          mma_commit(&kv_empty[seq % RING]);
-          ++seq;
+          mma_commit(&kv_empty[vslot]);
+          if (more) {
+            mma_commit(&kv_empty[slot]);
+            advance();
+          }
         }
       }
       mma_commit(mma_done);  // every MMA issued here completes before TMEM is released
       mbar_drain(mma_done, 0, err, kDevTimeoutDrain);
+    }
+    if (warp == 1) {
+      // ------------------------------------------------------------------ table walker: eight lanes, 16 keys each
+      uint32_t tile = 0;
+      bool ok = true;
+      Segment s;
+      while (ok && next_segment(a, wk, walk, s)) {
+        int64_t key = s.sl.lo + (int64_t)s.t0 * BN + lane * 16;
+        for (int j = s.t0; j < s.t1; ++j, ++tile, key += BN) {
+          const int64_t page = lane < 8 && key < s.sl.hi ? kv_page(a.c, a.s, s.sl.b, key >> a.c.page_log2) : -1;
+          int64_t off = -1;
+          float4 c = make_float4(0.f, -INFINITY, 0.f, 0.f);
+          if (page >= 0) {
+            const int64_t ph = page * a.c.kv_heads + s.kvh;
+            off = (ph * a.c.page + (key & (a.c.page - 1))) * D;
+            const float vs = fmaxf(__ldg(a.c.v_scale + ph), kKvScaleFloor);
+            c = make_float4(__ldg(a.c.k_scale + ph), kv_lg2(vs), __fdividef(1.f, vs), 0.f);
+          }
+          // entry tile - 8 is read once the decode warps may fill K of tile - 4: its ring slot held V of tile - 7, whose
+          // product is done
+          const uint32_t f = tile - 4;  // (a barrier a ring entry: the decode warps may be several tiles past f)
+          if (tile >= 4 && !__all_sync(0xffffffffu, mbar_wait_prompt(&wr_free[f % WR], (f / WR) & 1, abort_flag, err,
+                                                                      kDevTimeoutEmpty))) {
+            ok = false;
+            break;
+          }
+          if (lane < 8) {
+            consts[(tile % WR) * 8 + lane] = c;
+            addr[(tile % WR) * 8 + lane] = off;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&wr_full[tile % WR]);
+        }
+      }
     }
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_DEC));
@@ -284,45 +361,38 @@ __global__ void __launch_bounds__(THREADS, 1)
     constexpr int LPR = D / 16;                 // lanes to a K row
     constexpr int RPP = 128 / LPR;              // K rows of a pass of the four warps: 16 (D = 128) or 32
     constexpr int KP = BN / RPP;                // passes
-    constexpr int NV = D / 16;                  // words of a V row a thread takes: 4 (16 codes) or 2 ... see vq below
     const int krow = (dw * 32 + lane) / LPR, kch = lane % LPR;
     // V: eight keys (octet vo of the tile) and D / 8 columns (chunk vc) a thread
     const int vo = (lane & 7) + 8 * (dw >> 1), vc = (lane >> 3) + 4 * (dw & 1);
     constexpr int VW = D / 32;                  // words of a chunk
-    (void)NV;
     uint4 kbuf[KP];
     uint32_t vbuf[8][VW];
-    uint32_t seq = 0, tile = 0;
+    uint32_t seq = 0, tile0 = 0;
     bool ok = true;
     Segment s;
     while (ok && next_segment(a, wk, walk, s)) {
       const int n = s.t1 - s.t0;
       const int64_t key_base = s.sl.lo + (int64_t)s.t0 * BN;
-      // page of the 16 keys at `key`, -1 where the item has none
-      auto page_of = [&](int64_t key) -> int64_t {
-        return key < s.sl.hi ? kv_page(a.c, a.s, s.sl.b, key >> a.c.page_log2) : -1;
-      };
       auto load_k = [&](int j) {
-        int64_t off[KP];
+        const uint32_t T = tile0 + j;
+        if (!__all_sync(0xffffffffu, mbar_wait_prompt(&wr_full[T % WR], (T / WR) & 1, abort_flag, err, kDevTimeoutScale)))
+          return false;
 #pragma unroll
         for (int p = 0; p < KP; ++p) {
-          const int64_t key = key_base + (int64_t)j * BN + p * RPP + krow;
-          const int64_t page = page_of(key & ~(int64_t)15);
-          off[p] = page < 0 ? -1 : ((page * a.c.kv_heads + s.kvh) * a.c.page + (key & (a.c.page - 1))) * D + kch * 16;
+          const int row = p * RPP + krow;
+          const int64_t off = addr[(T % WR) * 8 + (row >> 4)];
+          kbuf[p] = off < 0 ? make_uint4(0, 0, 0, 0)
+                            : __ldg(reinterpret_cast<const uint4*>(a.c.k + off + (row & 15) * D + kch * 16));
         }
-#pragma unroll
-        for (int p = 0; p < KP; ++p)
-          kbuf[p] = off[p] < 0 ? make_uint4(0, 0, 0, 0) : __ldg(reinterpret_cast<const uint4*>(a.c.k + off[p]));
+        return true;
       };
       auto load_v = [&](int j) {
-        const int64_t key = key_base + (int64_t)j * BN + vo * 8;
-        const int64_t page = page_of(key & ~(int64_t)15);
-        const int64_t left = s.sl.len - key;  // what lies behind the last token may be any bits
-        const uint8_t* src =
-            a.c.v + (page < 0 ? 0 : ((page * a.c.kv_heads + s.kvh) * a.c.page + (key & (a.c.page - 1))) * D + vc * (D / 8));
+        const int64_t off = addr[((tile0 + j) % WR) * 8 + (vo >> 1)];
+        const int64_t left = s.sl.len - (key_base + (int64_t)j * BN + vo * 8);  // what lies behind the last token may be any bits
+        const uint8_t* src = a.c.v + (off < 0 ? 0 : off + (vo & 1) * 8 * D + vc * (D / 8));
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          const bool there = page >= 0 && r < left;
+          const bool there = off >= 0 && r < left;
           if (VW == 4) {
             const uint4 v = there ? __ldg(reinterpret_cast<const uint4*>(src + r * D)) : make_uint4(0, 0, 0, 0);
             vbuf[r][0] = v.x;
@@ -337,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       };
       auto wait_slot = [&]() {
-        return __all_sync(0xffffffffu, mbar_wait_bounded(&kv_empty[seq % RING], ((seq / RING) & 1) ^ 1, abort_flag, err,
+        return __all_sync(0xffffffffu, mbar_wait_prompt(&kv_empty[seq % RING], ((seq / RING) & 1) ^ 1, abort_flag, err,
                                                          kDevTimeoutEmpty));
       };
       auto publish = [&]() {
@@ -348,6 +418,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       auto put_k = [&](int j) {
         if (!wait_slot()) return false;
+        if (lane == 0) mbar_arrive(&wr_free[(tile0 + j) % WR]);
         const uint32_t dst = smem_u32(smem + C::OFF_KV + (seq % RING) * C::KV_TILE);
 #pragma unroll
         for (int p = 0; p < KP; ++p) {
@@ -361,20 +432,6 @@ __global__ void __launch_bounds__(THREADS, 1)
           sts128(rb + ((ch ^ (row & 7)) << 4), h[0], h[1], h[2], h[3]);
           sts128(rb + (((ch + 1) ^ (row & 7)) << 4), h[4], h[5], h[6], h[7]);
         }
-        if (dw == 0) {  // the scales of the tile's eight 16-key groups
-          if (lane < 8) {
-            const int64_t page = page_of(key_base + (int64_t)j * BN + lane * 16);
-            float4 c = make_float4(0.f, -INFINITY, 0.f, 0.f);
-            if (page >= 0) {
-              const float vs = fmaxf(__ldg(a.c.v_scale + page * a.c.kv_heads + s.kvh), kKvScaleFloor);
-              c = make_float4(__ldg(a.c.k_scale + page * a.c.kv_heads + s.kvh), kv_lg2(vs), __fdividef(1.f, vs), 0.f);
-            }
-            consts[(tile % SC) * 8 + lane] = c;
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sc_full[tile % SC]);
-        }
-        ++tile;
         publish();
         return true;
       };
@@ -398,20 +455,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         publish();
         return true;
       };
-      load_k(0);
-      ok = put_k(0);
-      if (!ok) break;
-      if (n > 1) load_k(1);
+      if (!(ok = load_k(0))) break;
       load_v(0);
-      for (int j = 0; ok && j < n; ++j) {
-        if (j + 1 < n) {
-          ok = put_k(j + 1);
-          if (!ok) break;
-          if (j + 2 < n) load_k(j + 2);
-        }
-        ok = put_v();
-        if (ok && j + 1 < n) load_v(j + 1);
+      for (int j = 0; j < n; ++j) {
+        if (!(ok = put_k(j))) break;
+        if (j + 1 < n && !(ok = load_k(j + 1))) break;
+        if (!(ok = put_v())) break;
+        if (j + 1 < n) load_v(j + 1);
       }
+      tile0 += n;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFT));
@@ -422,10 +474,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem_base + lane_off + g * BN;
     const uint32_t tO = tmem_base + lane_off + NQ * BN + g * D;
-    const uint32_t prow = smem_u32(smem + C::OFF_P + g * C::P_TILE) + rloc * 128;
     const uint32_t qrow = smem_u32(smem + g * C::Q_TILE) + rloc * 128;
     const uint32_t swz = rloc & 7;
-    uint32_t done = 0, tile0 = 0;
+    uint32_t done = 0, segs = 0, tile0 = 0;
     bool ok = true, first = true;
     Segment s;
     while (ok && next_segment(a, wk, walk, s)) {
@@ -496,51 +547,55 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[g]);
       }
+      const int64_t ro = in ? kv_row_out(a, s.sl, s.kvh, r) : 0;
       const int64_t key_base = s.sl.lo + (int64_t)s.t0 * BN;
-      int64_t lo = 0, hi = 0;
-      if (in) kv_row_keys(a, s.sl, r, lo, hi);
-      lo -= key_base;
-      hi -= key_base;
+      int64_t lo = 0, hi = s.sl.hi;
+      if (in) kv_row_keys(a, s.sl, r, lo, hi);  // a row that is not there sees all: its warp is spared the mask
+      const int64_t span = (int64_t)n * BN;
+      const int klo = (int)(lo < key_base ? 0 : (lo - key_base < span ? lo - key_base : span));
+      const int khi = (int)(hi < key_base ? 0 : (hi - key_base < span ? hi - key_base : span));
+      // the tiles that every row of the warp sees whole
+      const int full_lo = __reduce_max_sync(0xffffffffu, klo), full_hi = __reduce_min_sync(0xffffffffu, khi);
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j) {
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&s_full[g], done & 1, abort_flag, err, kDevTimeoutScores))) {
+        const uint32_t T = tile0 + j;
+        // (the ring only after the scores: a group that sat out slots may not look at it before it has come to them)
+        if (!__all_sync(0xffffffffu, mbar_wait_prompt(&s_full[g], done & 1, abort_flag, err, kDevTimeoutScores)) ||
+            !__all_sync(0xffffffffu,
+                        mbar_wait_prompt(&wr_full[T % WR], (T / WR) & 1, abort_flag, err, kDevTimeoutScale))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        uint32_t sr[BN / 32][32];
+        // The row's scores pass through registers 32 at a time, twice: for the maximum and for the weights.  Small
+        // loops: two softmax warps and a decode warp share an instruction cache, and straight-line code for 128
+        // scores is fetched more slowly than it runs.
+        const float4* cs = consts + (T % WR) * 8;
+        const int k0 = j * BN;
+        const bool edge = k0 < full_lo || k0 + BN > full_hi;  // some row does not see the whole tile
+        const int a0 = klo - k0, a1 = khi - k0;
+        uint32_t x[4][32];
 #pragma unroll
-        for (int k = 0; k < BN / 32; ++k) tmem_ld_32x32b_x32(tS + 32 * k, sr[k]);
+        for (int k = 0; k < 4; ++k) tmem_ld_32x32b_x32(tS + 32 * k, x[k]);
+        float4 cq[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) cq[q] = cs[q];
         tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[g]);
-        const uint32_t T = tile0 + j;
-        if (!__all_sync(0xffffffffu,
-                        mbar_wait_bounded(&sc_full[T % SC], (T / SC) & 1, abort_flag, err, kDevTimeoutScale))) {
-          ok = false;
-          break;
-        }
-        const float4* cs = consts + (T % SC) * 8;
-        const int64_t k0 = (int64_t)j * BN;
-        if (__any_sync(0xffffffffu, lo > k0 || hi < k0 + BN)) {  // some row does not see the whole tile
-          const int a0 = (int)(lo - k0 < 0 ? 0 : (lo - k0 > BN ? BN : lo - k0));
-          const int a1 = (int)(hi - k0 < 0 ? 0 : (hi - k0 > BN ? BN : hi - k0));
+        if (edge) {
 #pragma unroll
           for (int i = 0; i < BN; ++i)
-            if (i < a0 || i >= a1) sr[i >> 5][i & 31] = 0xff800000u;
+            if (i < a0 || i >= a1) x[i >> 5][i & 31] = 0xff800000u;
         }
         float mx = -INFINITY;
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          float mg[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            mg[i & 1] = max3f(mg[i & 1], __uint_as_float(sr[q >> 1][(q & 1) * 16 + 2 * i]),
-                              __uint_as_float(sr[q >> 1][(q & 1) * 16 + 2 * i + 1]));
-          const float4 cq = cs[q];
-          // at least 1e-37, so that a masked -inf stays -inf for a scale of 0
-          mx = fmaxf(mx, __fmaf_rn(fmaxf(mg[0], mg[1]), fmaxf(c * cq.x, 1e-37f), cq.y));
+          const uint32_t* v = &x[q >> 1][(q & 1) * 16];
+          auto f = [&](int i) { return __uint_as_float(v[i]); };
+          const float u0 = max3f(f(0), f(1), f(2)), u1 = max3f(f(3), f(4), f(5)), u2 = max3f(f(6), f(7), f(8)),
+                      u3 = max3f(f(9), f(10), f(11)), u4 = max3f(f(12), f(13), f(14));
+          // the factor is not 0, so that a masked -inf stays -inf for a scale of 0
+          cq[q].x = fmaxf(c * cq[q].x, 1e-37f);
+          mx = fmaxf(mx, __fmaf_rn(fmaxf(max3f(u0, u1, u2), max3f(u3, u4, f(15))), cq[q].x, cq[q].y));
         }
         const bool move = mx > m_used + kMove;
         float alpha = 1.f;
@@ -550,57 +605,42 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         l *= alpha;
         const float m = m_used == -INFINITY ? 0.f : m_used;
-        uint32_t pk16[BN / 2];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float4 cq = cs[q];
-          const float ck = fmaxf(c * cq.x, 1e-37f), off = cq.y - m;
-          const f2 c2 = pk(ck, ck), o2 = pk(off, off);
-          f2 la = pk(0.f, 0.f);
+        for (int k = 0; k < 4; ++k) {
+          uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float t0, t1;
-            upk(fma2(pk(__uint_as_float(sr[q >> 1][(q & 1) * 16 + 2 * i]),
-                        __uint_as_float(sr[q >> 1][(q & 1) * 16 + 2 * i + 1])),
-                     c2, o2),
-                t0, t1);
-            const float p0 = kv_ex2(t0), p1 = kv_ex2(t1);
-            la = add2(la, pk(p0, p1));
-            pk16[q * 8 + i] = kv_pack_f16(p0, p1);
-          }
-          float s0, s1;
-          upk(la, s0, s1);
-          l = __fmaf_rn(s0 + s1, cq.z, l);
-        }
-        // W_g and O_g are free once the previous tile's product has completed
-        if (j > 0) {
-          if (!__all_sync(0xffffffffu,
-                          mbar_wait_bounded(&pv_done[g], (done - 1) & 1, abort_flag, err, kDevTimeoutPV))) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          if (__any_sync(0xffffffffu, move)) {
-#pragma unroll 1
-            for (int k = 0; k < D / 32; ++k) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(tO + 32 * k, o);
-              tmem_wait_ld();
+          for (int h = 0; h < 2; ++h) {
+            const int q = 2 * k + h;
+            const float off = cq[q].y - m;
+            const f2 c2 = pk(cq[q].x, cq[q].x), o2 = pk(off, off);
+            f2 la = pk(0.f, 0.f);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st_32x32b_x32(tO + 32 * k, o);
+            for (int i = 0; i < 8; ++i) {
+              float t0, t1;
+              upk(fma2(pk(__uint_as_float(x[k][h * 16 + 2 * i]), __uint_as_float(x[k][h * 16 + 2 * i + 1])), c2, o2), t0, t1);
+              const float p0 = kv_ex2(t0), p1 = kv_ex2(t1);
+              la = add2(la, pk(p0, p1));
+              w[h * 8 + i] = kv_pack_f16(p0, p1);
             }
-            tmem_wait_st();
+            float s0, s1;
+            upk(la, s0, s1);
+            l = __fmaf_rn(s0 + s1, cs[q].z, l);
+          }
+          tmem_st_32x32b_x16(tS + 16 * k, w);
+        }
+        // O_g holds every product before these scores
+        if (j > 0 && __any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+          for (int k = 0; k < D / 16; ++k) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(tO + 16 * k, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st_32x32b_x16(tO + 16 * k, o);
           }
         }
-#pragma unroll
-        for (int sl = 0; sl < 2; ++sl)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint32_t* q4 = &pk16[sl * 32 + k * 4];
-            sts128(prow + sl * C::P_SLAB + ((k ^ swz) << 4), q4[0], q4[1], q4[2], q4[3]);
-          }
-        fence_proxy_async_smem();
+        tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[g]);
@@ -608,12 +648,11 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (!ok) break;
       tile0 += n;
-      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&pv_done[g], (done - 1) & 1, abort_flag, err, kDevTimeoutPV))) {
+      if (!__all_sync(0xffffffffu, mbar_wait_prompt(&o_full[g], segs++ & 1, abort_flag, err, kDevTimeoutPV))) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const int64_t ro = in ? kv_row_out(a, s.sl, s.kvh, r) : 0;
       float* part = a.part + (int64_t)part_slot * ROWS * (D + 2);
       const float inv = l > 0.f ? __fdiv_rn(1.f, l) : (l == 0.f ? 0.f : l);  // a NaN goes through
 #pragma unroll 1
