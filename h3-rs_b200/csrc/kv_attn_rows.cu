@@ -28,7 +28,7 @@ constexpr float kMove = 8.f;        // log2 of the largest weight between moves 
 
 template <int D, int MT>
 struct RowsCfg {
-  static constexpr int kStages = MT == 1 ? 3 : 6;
+  static constexpr int kStages = MT == 1 ? 3 : 5;
   static constexpr int kStageBytes = 2 * 16 * D;           // K and V codes of 16 keys
   static constexpr int kRing = kStages * kStageBytes;      // a warp's ring; its O of 16 MT rows fits there too
   static constexpr int kQBytes = MT * 16 * D * 2;
@@ -36,8 +36,8 @@ struct RowsCfg {
   static_assert(kRing >= MT * 16 * D * 4, "the ring holds a warp's partial output");
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -118,7 +118,7 @@ __device__ __forceinline__ int sched_load(const KvAttnArgs& a, Sched& sc, int64_
 template <int D, int CODES, int MT>
 __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel(const KvAttnArgs a) {
   using C = RowsCfg<D, MT>;
-  constexpr int TILE = MT * 16, NT = D / 8, KS = D / 16;
+  constexpr int TILE = MT * 16, NT = D / 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Sched sc;
   __shared__ float row_c[TILE];                   // c of the row: scale * log2 e and the power of two taken out of q
@@ -156,6 +156,17 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
   __syncthreads();
   int li = sc.found;
   bool first_segment = true;
+  const int group_log2 = a.c.page_log2 - 4, group_mask = (1 << group_log2) - 1;  // 16-key groups of a page
+  const uint32_t pool = (uint32_t)a.c.pages;
+  const int64_t page_bytes = (int64_t)a.c.kv_heads * a.c.page * D;
+  // Places in a 16-key tile.  Copies: lane's 16-byte piece of rows lane / (D / 16) + 32 i / (D / 16).
+  const uint32_t cp_off[2] = {tile_off<D>(lane / (D / 16), lane % (D / 16)),
+                              tile_off<D>((lane + 32) / (D / 16), (lane + 32) % (D / 16))};
+  // K: codes 32 t .. of key g (D = 128; the second 16 bytes are the place with bit 4 flipped) or 16 t .. (D = 64).
+  const uint32_t k_off = tile_off<D>(g, t4 * (D / 64));
+  // V: codes (D / 8) g .. of key 2 t; key 2 t + 1 is beside it, keys 2 t + 8 and + 9 eight rows on.
+  const uint32_t v_off0 = tile_off<D>(2 * t4, g * (D / 8) / 16) + (g * (D / 8)) % 16;
+  const uint32_t v_off1 = tile_off<D>(2 * t4 + 1, g * (D / 8) / 16) + (g * (D / 8)) % 16;
 
   while (true) {
     // ---------------------------------------------------------------- the segment: units [u0, u1) of (slot, kvh)
@@ -171,34 +182,48 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
     const int64_t key1 = sl.lo + (int64_t)u1 * kUnit < sl.hi ? sl.lo + (int64_t)u1 * kUnit : sl.hi;
     const int steps_all = (int)((key1 - key0 + 15) / 16);
     const int steps = steps_all > warp ? (steps_all - warp + kWarps - 1) / kWarps : 0;
-    const int64_t group0 = key0 / 16 + warp;
+    const int group0 = (int)(key0 / 16) + warp;
+    const int32_t* table = a.s.table + (int64_t)sl.b * a.s.width;
+    const float* k_scale = a.c.k_scale + kvh;
+    const float* v_scale = a.c.v_scale + kvh;
 
-    auto page_of = [&](int st) -> int64_t {
-      return st < steps ? kv_page(a.c, a.s, sl.b, ((group0 + (int64_t)st * kWarps) * 16) >> a.c.page_log2) : -1;
+    // page of step st or of the last one, -1 where the table names none (keys below sl.hi lie within the table's width;
+    // a warp without a step looks at the item's first page)
+    auto page_of = [&](int st) -> int {
+      const int grp = steps > 0 ? group0 + min(st, steps - 1) * kWarps : group0 - warp;
+      const int p = __ldg(table + (grp >> group_log2));
+      return (uint32_t)p < pool ? p : -1;
     };
-    auto issue = [&](int st, int64_t page) {
-      if (st < steps) {
-        const bool there = page >= 0;
-        const int64_t key = (group0 + (int64_t)st * kWarps) * 16;
-        const int64_t off =
-            there ? ((page * a.c.kv_heads + kvh) * a.c.page + (key & (a.c.page - 1))) * D : 0;
-        const uint32_t dst = ring_u + (st % C::kStages) * C::kStageBytes;
+    auto issue = [&](int st, int page, uint32_t dst) {
+      if (page >= 0 && st < steps) {
+        const int64_t off = page * page_bytes + (int64_t)(((kvh << group_log2) + ((group0 + st * kWarps) & group_mask)) * (16 * D)) + lane * 16;
+        const uint8_t* ks = a.c.k + off;
+        const uint8_t* vs = a.c.v + off;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
-          const int ch = lane + 32 * i;
-          const uint32_t o = tile_off<D>(ch / (D / 16), ch % (D / 16));
-          cp16(dst + o, a.c.k + off + ch * 16, there);
-          cp16(dst + 16 * D + o, a.c.v + off + ch * 16, there);
+          const uint32_t o = dst + cp_off[i & 1] + (i >> 1) * 1024;
+          cp16(o, ks + i * 512);
+          cp16(o + 16 * D, vs + i * 512);
         }
       }
       cp_commit();
     };
 
-    int64_t pages[C::kStages];  // pages of the steps in flight; [0]: the step consumed next
+    int pages[C::kStages + 1];  // pages of the steps from the one consumed next on
 #pragma unroll
-    for (int i = 0; i < C::kStages; ++i) pages[i] = page_of(i);
+    for (int i = 0; i <= C::kStages; ++i) pages[i] = page_of(i);
+    uint32_t cur = ring_u, put = ring_u;
+    auto next = [&](uint32_t& x) {
+      x += C::kStageBytes;
+      if (x == ring_u + C::kRing) x = ring_u;
+    };
 #pragma unroll
-    for (int i = 0; i < C::kStages - 1; ++i) issue(i, pages[i]);
+    for (int i = 0; i < C::kStages - 1; ++i) {
+      issue(i, pages[i], put);
+      next(put);
+    }
+    auto scale_of = [&](const float* s, int page) { return __ldg(s + (int64_t)max(page, 0) * a.c.kv_heads); };
+    float ks_next = scale_of(k_scale, pages[0]), vs_next = scale_of(v_scale, pages[0]);
 
     // ---------------------------------------------------------------- q: f16 in the order of the A fragments
     for (int r = warp; r < TILE; r += kWarps) {
@@ -226,12 +251,13 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
         }
       }
       if (lane == 0) row_c[r] = c;
-      // element d of the row: lane t = d / (D / 4) of the quad, its element e = d % (D / 4); pair of k-steps e / 8
+      // element d of the row: lane t = d / (D / 4) of the quad, its element e = d % (D / 4), k-step e / 4; the four
+      // registers of a fragment are (row g, first pair), (row g + 8, first), (row g, second), (row g + 8, second)
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         const int d = lane + 32 * i, tt = d / (D / 4), e = d % (D / 4);
         const int mt = r >> 4, half = (r >> 3) & 1, gg = r & 7;
-        const uint32_t o = (uint32_t)((((mt * (D / 32) + e / 8) * 2 + half) * 32 + gg * 4 + tt) * 16 + (e % 8) * 2);
+        const uint32_t o = (uint32_t)(((mt * (D / 16) + e / 4) * 32 + gg * 4 + tt) * 16 + ((e & 2) + half) * 4 + (e & 1) * 2);
         asm volatile("st.shared.b16 [%0], %1;" ::"r"(q_u + o), "h"(f2h(f[i])) : "memory");
       }
     }
@@ -262,22 +288,28 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
     }
     // keys of this segment that every row sees need no mask
     const int64_t pos0 = sl.len - sl.n + sl.r0 / a.per, pos1 = sl.len - sl.n + (sl.r0 + sl.rows - 1) / a.per;
-    const int64_t all_hi = (a.causal && pos0 + 1 < sl.len ? pos0 + 1 : sl.len) - key0;
-    const int64_t all_lo = (a.window > 0 && pos1 + 1 > a.window ? pos1 + 1 - a.window : 0) - key0;
+    const int64_t all_hi64 = (a.causal && pos0 + 1 < sl.len ? pos0 + 1 : sl.len) - key0;
+    const int64_t all_lo64 = (a.window > 0 && pos1 + 1 > a.window ? pos1 + 1 - a.window : 0) - key0;
+    const int all_hi = (int)(all_hi64 < 0 ? 0 : (all_hi64 > 0x3fffffff ? 0x3fffffff : all_hi64));
+    const int all_lo = (int)(all_lo64 < 0 ? 0 : (all_lo64 > 0x3fffffff ? 0x3fffffff : all_lo64));
+    const int left_all = sl.len - key0 > 0x3fffffff ? 0x3fffffff : (int)(sl.len - key0);
 
-    for (int st = 0; st < steps; ++st) {
+    int rel = warp * 16;  // first key of the step, relative to key0
+    for (int st = 0; st < steps; ++st, rel += kUnit) {
       cp_wait<C::kStages - 2>();
       __syncwarp();
-      issue(st + C::kStages - 1, pages[C::kStages - 1]);
-      const int64_t page = pages[0];
+      issue(st + C::kStages - 1, pages[C::kStages - 1], put);
+      next(put);
+      const int page = pages[0];
+      const float ks = ks_next, vs = fmaxf(vs_next, kKvScaleFloor);
 #pragma unroll
-      for (int i = 0; i + 1 < C::kStages; ++i) pages[i] = pages[i + 1];
-      pages[C::kStages - 1] = page_of(st + C::kStages);
+      for (int i = 0; i < C::kStages; ++i) pages[i] = pages[i + 1];
+      pages[C::kStages] = page_of(st + C::kStages + 1);
+      ks_next = scale_of(k_scale, pages[0]);
+      vs_next = scale_of(v_scale, pages[0]);
+      const uint32_t kt = cur, vt = cur + 16 * D;
+      next(cur);
       if (page < 0) continue;
-      const float ks = __ldg(a.c.k_scale + page * a.c.kv_heads + kvh);
-      const float vs = fmaxf(__ldg(a.c.v_scale + page * a.c.kv_heads + kvh), kKvScaleFloor);
-      const uint32_t kt = ring_u + (st % C::kStages) * C::kStageBytes, vt = kt + 16 * D;
-      const int rel = (warp + st * kWarps) * 16;  // first key of the step, relative to key0
 
       // ------------------------------------------------------------ S = Q K^T: two 8-key tiles
       float s[MT][2][4];
@@ -288,29 +320,33 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
 #pragma unroll
-      for (int sp = 0; sp < KS / 2; ++sp) {  // two k-steps: 8 codes a lane and key
-        uint32_t kw[2][2];
+      for (int hb = 0; hb < D / 64; ++hb) {  // 16 codes a lane and key: four k-steps
+        uint32_t kw[2][4];
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt) {
-          const int row = nt * 8 + g, byte = t4 * (D / 4) + sp * 8;
-          const uint2 r = lds64(kt + tile_off<D>(row, byte >> 4) + (byte & 8));
+          const uint4 r = lds128((kt + nt * 8 * D + k_off) ^ (hb << 4));
           kw[nt][0] = r.x;
           kw[nt][1] = r.y;
-        }
-        uint32_t b[2][4];
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          kv_decode4<CODES>(kw[nt][0], b[nt][0], b[nt][1]);
-          kv_decode4<CODES>(kw[nt][1], b[nt][2], b[nt][3]);
+          kw[nt][2] = r.z;
+          kw[nt][3] = r.w;
         }
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const uint4 qa = lds128(q_u + (uint32_t)((((mt * (D / 32) + sp) * 2 + 0) * 32 + lane) * 16));
-          const uint4 qb = lds128(q_u + (uint32_t)((((mt * (D / 32) + sp) * 2 + 1) * 32 + lane) * 16));
+        for (int sp = 0; sp < 2; ++sp) {
+          uint32_t b[2][4];
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt) {
-            mma16816(s[mt][nt], qa.x, qb.x, qa.y, qb.y, b[nt][0], b[nt][1]);
-            mma16816(s[mt][nt], qa.z, qb.z, qa.w, qb.w, b[nt][2], b[nt][3]);
+            kv_decode4<CODES>(kw[nt][2 * sp], b[nt][0], b[nt][1]);
+            kv_decode4<CODES>(kw[nt][2 * sp + 1], b[nt][2], b[nt][3]);
+          }
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const uint32_t qo = q_u + (uint32_t)(((mt * (D / 16) + 4 * hb + 2 * sp) * 32 + lane) * 16);
+            const uint4 qa = lds128(qo), qb = lds128(qo + 512);
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+              mma16816(s[mt][nt], qa.x, qa.y, qa.z, qa.w, b[nt][0], b[nt][1]);
+              mma16816(s[mt][nt], qb.x, qb.y, qb.z, qb.w, b[nt][2], b[nt][3]);
+            }
           }
         }
       }
@@ -321,28 +357,32 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
       uint32_t pa[MT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        float tv[2][4];  // [row half][key]
+        float ck[2], tv[2][4];  // [row half][key]: t + log2 vs - m; before the first maximum (m = -inf) it is +inf
         bool up = false;
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          const float ck = cr[mt][hf] * ks;
-          float mx = -INFINITY;
+          ck[hf] = cr[mt][hf] * ks;
+          const float off = lv - m_run[mt][hf];
 #pragma unroll
-          for (int k4 = 0; k4 < 4; ++k4) {
-            float v = __fmaf_rn(s[mt][k4 >> 1][hf * 2 + (k4 & 1)], ck, lv);
-            if (edge) {
+          for (int k4 = 0; k4 < 4; ++k4) tv[hf][k4] = __fmaf_rn(s[mt][k4 >> 1][hf * 2 + (k4 & 1)], ck[hf], off);
+          if (edge) {
+#pragma unroll
+            for (int k4 = 0; k4 < 4; ++k4) {
               const int key = rel + (k4 >> 1) * 8 + 2 * t4 + (k4 & 1);
-              v = key >= rlo[mt][hf] && key < rhi[mt][hf] ? v : -INFINITY;
+              if (key < rlo[mt][hf] || key >= rhi[mt][hf]) tv[hf][k4] = -INFINITY;
             }
-            tv[hf][k4] = v;
-            mx = fmaxf(mx, v);
           }
-          up |= mx > m_run[mt][hf] + kMove;
+          up |= fmaxf(max3f(tv[hf][0], tv[hf][1], tv[hf][2]), tv[hf][3]) > kMove;
         }
         if (__any_sync(0xffffffffu, up)) {  // rare after the first steps: move the maximum of the rows that need it
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
-            float mx = fmaxf(fmaxf(tv[hf][0], tv[hf][1]), fmaxf(tv[hf][2], tv[hf][3]));
+            float t[4], mx = -INFINITY;
+#pragma unroll
+            for (int k4 = 0; k4 < 4; ++k4) {
+              t[k4] = tv[hf][k4] == -INFINITY ? -INFINITY : __fmaf_rn(s[mt][k4 >> 1][hf * 2 + (k4 & 1)], ck[hf], lv);
+              mx = fmaxf(mx, t[k4]);
+            }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             if (mx > m_run[mt][hf] + kMove) {
@@ -354,15 +394,16 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
                 o_acc[mt][j][2 * hf] *= f;
                 o_acc[mt][j][2 * hf + 1] *= f;
               }
+#pragma unroll
+              for (int k4 = 0; k4 < 4; ++k4) tv[hf][k4] = t[k4] - mx;
             }
           }
         }
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          const float m = m_run[mt][hf] == -INFINITY ? 0.f : m_run[mt][hf];
           float p[4];
 #pragma unroll
-          for (int k4 = 0; k4 < 4; ++k4) p[k4] = kv_ex2(tv[hf][k4] - m);
+          for (int k4 = 0; k4 < 4; ++k4) p[k4] = kv_ex2(tv[hf][k4]);
           l_run[mt][hf] = __fmaf_rn((p[0] + p[1]) + (p[2] + p[3]), iv, l_run[mt][hf]);
           pa[mt][hf] = kv_pack_f16(p[0], p[1]);
           pa[mt][2 + hf] = kv_pack_f16(p[2], p[3]);
@@ -370,16 +411,32 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
       }
 
       // ------------------------------------------------------------ O += W V
-      const int64_t left = sl.len - (key0 + rel);  // keys of this step that the sequence has
+      uint32_t vr[4][D / 32];
+#pragma unroll
+      for (int k4 = 0; k4 < 4; ++k4) {
+        const uint32_t at = vt + (k4 & 1 ? v_off1 : v_off0) + (k4 >> 1) * 8 * D;
+        if (D == 128) {
+          const uint4 r = lds128(at);
+          vr[k4][0] = r.x;
+          vr[k4][1] = r.y;
+          vr[k4][D / 32 - 2] = r.z;
+          vr[k4][D / 32 - 1] = r.w;
+        } else {
+          const uint2 r = lds64(at);
+          vr[k4][0] = r.x;
+          vr[k4][1] = r.y;
+        }
+      }
+      if (CODES == kKvE4m3 && left_all - rel < 16) {  // what lies behind the last token may be any bits, NaN among them
+#pragma unroll
+        for (int k4 = 0; k4 < 4; ++k4)
+          if ((k4 >> 1) * 8 + 2 * t4 + (k4 & 1) >= left_all - rel)
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) vr[k4][i] = 0;
+      }
 #pragma unroll
       for (int jq = 0; jq < NT / 4; ++jq) {  // 4 column tiles: one word of each of the lane's four keys
-        uint32_t vw[4];
-#pragma unroll
-        for (int k4 = 0; k4 < 4; ++k4) {
-          const int row = (k4 >> 1) * 8 + 2 * t4 + (k4 & 1), byte = g * (D / 8) + jq * 4;
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(vw[k4]) : "r"(vt + tile_off<D>(row, byte >> 4) + (byte & 12)) : "memory");
-          if (left < 16 && row >= left) vw[k4] = 0;  // what lies behind the last token may be any bits
-        }
+        const uint32_t vw[4] = {vr[0][jq], vr[1][jq], vr[2][jq], vr[3][jq]};
         uint32_t b0[4], b1[4];
         kv_decode4<CODES>(prmt(vw[0], vw[1], 0x5140), b0[0], b0[1]);
         kv_decode4<CODES>(prmt(vw[0], vw[1], 0x7362), b0[2], b0[3]);

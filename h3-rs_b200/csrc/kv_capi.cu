@@ -54,8 +54,8 @@ h3q_status check_cache(const h3q_kv_cache* c, const char* what) {
     return fail(H3Q_ERR_UNSUPPORTED, "%s: this build handles head_dim 64 and 128 (got %d)", what, c->head_dim);
   if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128)
     return fail(H3Q_ERR_UNSUPPORTED, "%s: this build handles pages of 16, 32, 64 or 128 tokens (got %d)", what, c->page);
-  if (c->kv_heads > 4096 || c->pages > (int64_t)1 << 31)
-    return fail(H3Q_ERR_UNSUPPORTED, "%s: this build handles up to 4096 kv heads and 2^31 pages", what);
+  if (c->kv_heads > 4096 || c->pages >= (int64_t)1 << 31)
+    return fail(H3Q_ERR_UNSUPPORTED, "%s: this build handles up to 4096 kv heads and less than 2^31 pages", what);
   if (c->pages > 0) {
     if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(H3Q_ERR_ARG, "%s: null cache pointer", what);
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->k_scale, 4) || !aligned(c->v_scale, 4))
@@ -228,7 +228,7 @@ h3q_status h3q_kv_attention(const h3q_kv_cache* cache, const void* q, int kind, 
   if (!aligned(workspace, 16)) return fail(H3Q_ERR_ARG, "%s: workspace must be 16-byte aligned", what);
   KvAttnArgs a{};
   a.c = cache_of(cache);
-  a.s = seqs_of(page_table, table_width, starts, batch, tokens);
+  a.s = seqs_of(page_table, cache->pages > 0 ? table_width : 0, starts, batch, tokens);  // no pages: no keys
   a.q = static_cast<const uint16_t*>(q);
   a.q_ts = q_token_stride;
   a.q_hs = q_head_stride;
