@@ -28,11 +28,16 @@ struct KvAttnArgs {
   uint16_t* out;           // [tokens, heads, dim]
   float* lse;              // [tokens, heads] or null
   int row_lo, row_hi;      // this launch takes the sequences whose rows (new tokens * per) are in (row_lo, row_hi]
+  int last;                // no launch takes sequences of more than row_hi rows
   int one;                 // every sequence of this launch has one slot, its own index
   int64_t slots;
-  float* part;             // partial results of split items
-  int4* meta;              // [slots * kv_heads]: first part, parts
+  // Items (a slot and kv head) are cut between workers (CTAs); worker w's parts are 2 w (its first segment) and 2 w + 1.
+  // A part is O of its rows, [rows][dim] (tiles of 16 and 32) or [dim / 4][rows][4] (tiles of 256), then (m, l) a row.
+  float* part;
+  int4* meta;              // [workers]: slot, kv head, first part and parts of the item that w began and did not finish
+  int workers;
 };
+constexpr int kMaxWorkers = 256;  // one a multiprocessor
 
 // What a slot stands for: `rows` query rows of sequence b, (token, head of the group) in that order, and the keys
 // [lo, hi) that any of them sees, lo a multiple of 16.
@@ -43,7 +48,7 @@ struct KvSlot {
 
 __device__ __forceinline__ bool kv_slot(const KvAttnArgs& a, int64_t slot, int b, int tile, KvSlot& t) {
   const int s0 = kv_start(a.s, b), n = kv_start(a.s, b + 1) - s0;
-  const int64_t all = (int64_t)n * a.per;
+  const int64_t all = (int64_t)n * a.per;  // at most 2^30 (checked by the host)
   t.rows = 0;
   t.lo = t.hi = 0;
   if (n <= 0 || all <= a.row_lo || all > a.row_hi) return false;
@@ -58,7 +63,7 @@ __device__ __forceinline__ bool kv_slot(const KvAttnArgs& a, int64_t slot, int b
   const int64_t most = a.s.width << a.c.page_log2;
   len = len < 0 ? 0 : (len > most ? most : len);
   t.len = len;
-  const int64_t first = len - n + r0 / a.per, last = len - n + (r0 + t.rows - 1) / a.per;
+  const int64_t first = len - n + t.r0 / a.per, last = len - n + (t.r0 + t.rows - 1) / a.per;
   int64_t hi = a.causal ? (last + 1 < len ? last + 1 : len) : len;
   int64_t lo = a.window > 0 && first + 1 > a.window ? first + 1 - a.window : 0;
   hi = hi < 0 ? 0 : hi;
@@ -78,6 +83,16 @@ __device__ __forceinline__ void kv_row_keys(const KvAttnArgs& a, const KvSlot& t
 __device__ __forceinline__ int64_t kv_row_out(const KvAttnArgs& a, const KvSlot& t, int kvh, int r) {
   const int rr = t.r0 + r;
   return (int64_t)(t.s0 + rr / a.per) * a.heads + kvh * a.per + rr % a.per;
+}
+
+// four columns (chunk ch) of output row ro, from the unnormalised sums and the row's statistics
+__device__ __forceinline__ void kv_put_row(const KvAttnArgs& a, int64_t ro, int ch, int dim, float4 o, float m, float l) {
+  const float inv = l > 0.f ? __fdiv_rn(1.f, l) : (l == 0.f ? 0.f : l);  // no key: zeros; a NaN goes through
+  uint2 w;
+  w.x = kv_pack(o.x * inv, o.y * inv, a.kind);
+  w.y = kv_pack(o.z * inv, o.w * inv, a.kind);
+  *reinterpret_cast<uint2*>(a.out + ro * dim + ch * 4) = w;
+  if (a.lse && ch == 0) a.lse[ro] = l == 0.f ? -INFINITY : 0.6931471805599453f * (m + log2f(l));
 }
 
 // joins the parts of items that were cut between CTAs, and writes the rows of slots without keys

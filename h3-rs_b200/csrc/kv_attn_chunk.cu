@@ -201,7 +201,10 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t all = wk.head[1], workers = all < gridDim.x ? all : gridDim.x;
-  if (blockIdx.x >= workers) return;
+  if (blockIdx.x >= workers) {
+    if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
   Walk walk{all * blockIdx.x / workers, all * (blockIdx.x + 1) / workers, 0};
   if (threadIdx.x == 0) {
     for (int i = 0; i < RING; ++i) { mbar_init(&kv_full[i], 4); mbar_init(&kv_empty[i], 1); }
@@ -484,10 +487,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool whole = s.t0 == 0 && s.t1 == s.e.tiles;
       const int part_slot = (int)blockIdx.x * 2 + (first ? 0 : 1);
       first = false;
-      if (s.t0 == 0 && g == 0 && rloc == 0) {
-        const int64_t y = s.e.before + (int64_t)(s.kvh + 1) * s.e.tiles - 1;
-        const int64_t w1 = ((y + 1) * workers - 1) / all;
-        a.meta[(int64_t)s.e.slot * a.c.kv_heads + s.kvh] = make_int4(part_slot, (int)(w1 - blockIdx.x) + 1, (int)blockIdx.x, 0);
+      if (g == 0 && rloc == 0) {
+        if (s.t0 == 0 && !whole) {
+          const int64_t y = s.e.before + (int64_t)(s.kvh + 1) * s.e.tiles - 1;
+          const int64_t w1 = ((y + 1) * workers - 1) / all;
+          a.meta[blockIdx.x] = make_int4(s.e.slot, s.kvh, part_slot, (int)(w1 - blockIdx.x) + 1);
+        } else if (walk.x >= walk.end) {  // the last segment, and not one that others go on with
+          a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+        }
       }
       if (g * BM >= s.sl.rows) {  // a slot of one tile
         tile0 += n;
@@ -672,9 +679,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             d4[i] = make_uint4(w[0], w[1], w[2], w[3]);
           }
         } else {
-          uint4* d4 = reinterpret_cast<uint4*>(part + (int64_t)r * D + 32 * k);
+          uint4* d4 = reinterpret_cast<uint4*>(part) + (int64_t)(8 * k) * ROWS + r;  // a warp's rows are neighbours
 #pragma unroll
-          for (int i = 0; i < 8; ++i) d4[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < 8; ++i) d4[i * ROWS] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
       }
       if (in) {
@@ -696,7 +703,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 namespace {
 
 template <int D, int CODES>
-cudaError_t launch_chunk(const KvAttnArgs& a, const KvChunkWork& wk, int q_vec, int* err, cudaStream_t st) {
+cudaError_t launch_chunk(KvAttnArgs a, const KvChunkWork& wk, int q_vec, int* err, cudaStream_t st) {
   auto kern = kv_attn_chunk_kernel<D, CODES>;
   static bool ready[64] = {false};
   int dev = 0;
@@ -709,14 +716,15 @@ cudaError_t launch_chunk(const KvAttnArgs& a, const KvChunkWork& wk, int q_vec, 
   }
   kv_attn_list_kernel<<<1, 1024, 0, st>>>(a, wk);
   if (const cudaError_t e = cudaGetLastError()) return e;
-  kern<<<(unsigned)sm_count(dev), THREADS, Cfg<D>::SMEM, st>>>(a, wk, q_vec, err);
+  a.workers = sm_count(dev);
+  kern<<<(unsigned)a.workers, THREADS, Cfg<D>::SMEM, st>>>(a, wk, q_vec, err);
   if (const cudaError_t e = cudaGetLastError()) return e;
   return launch_kv_attn_join(a, ROWS, st);
 }
 
 }  // namespace
 
-size_t kv_attn_chunk_part_bytes(int dim) { return (size_t)sm_count(0) * 2 * ROWS * (dim + 2) * 4; }
+size_t kv_attn_chunk_part_bytes(int dim) { return (size_t)kMaxWorkers * 2 * ROWS * (dim + 2) * 4; }
 size_t kv_attn_chunk_list_bytes(int64_t slots) { return 256 + (size_t)slots * sizeof(KvListed); }
 
 cudaError_t launch_kv_attn_chunk(const KvAttnArgs& a, void* list, int* err, cudaStream_t st) {

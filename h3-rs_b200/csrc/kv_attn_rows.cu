@@ -22,13 +22,13 @@ namespace h3q {
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
-constexpr int kUnit = kWarps * 16;  // keys of a unit
 constexpr float kMove = 8.f;        // log2 of the largest weight between moves of the running maximum
 
 template <int D, int MT>
 struct RowsCfg {
-  static constexpr int kStages = MT == 1 ? 3 : 5;
+  static constexpr int kWarps = MT == 1 ? 12 : 8, kThreads = kWarps * 32;
+  static constexpr int kUnit = kWarps * 16;  // keys of a unit
+  static constexpr int kStages = MT == 1 ? 3 : 4;
   static constexpr int kStageBytes = 2 * 16 * D;           // K and V codes of 16 keys
   static constexpr int kRing = kStages * kStageBytes;      // a warp's ring; its O of 16 MT rows fits there too
   static constexpr int kQBytes = MT * 16 * D * 2;
@@ -71,28 +71,31 @@ __device__ __forceinline__ uint32_t tile_off(int row, int ch) {
 
 // The units of the call in order, and this CTA's place in them: the units of kThreads slots at a time in shared
 // memory with their running sum.
+template <int W>
 struct Sched {
+  static constexpr int kWarps = W, kThreads = W * 32;
   int units[kThreads], pre[kThreads], seq[kThreads];
   int warp_sum[kWarps];
   int found;
 };
 
-template <int TILE>
+template <int TILE, int UNIT>
 __device__ __forceinline__ int slot_units(const KvAttnArgs& a, int64_t slot, int& b) {
   b = 0;
   if (slot >= a.slots) return 0;
   b = a.one ? (int)slot : kv_slot_seq(a.s, slot, a.per, TILE, 1);
   KvSlot t;
   if (!kv_slot(a, slot, b, TILE, t)) return 0;
-  return (int)((t.hi - t.lo + kUnit - 1) / kUnit);
+  return (int)((t.hi - t.lo + UNIT - 1) / UNIT);
 }
 
 // Fills `sc` with the slots from `base` on; returns the sum of their units.  All threads of the CTA.
-template <int TILE>
-__device__ __forceinline__ int sched_load(const KvAttnArgs& a, Sched& sc, int64_t base) {
+template <int TILE, int W>
+__device__ __forceinline__ int sched_load(const KvAttnArgs& a, Sched<W>& sc, int64_t base) {
+  constexpr int kWarps = W;
   __syncthreads();
   int b;
-  const int u = slot_units<TILE>(a, base + threadIdx.x, b);
+  const int u = slot_units<TILE, W * 16>(a, base + threadIdx.x, b);
   int x = u;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -116,13 +119,13 @@ __device__ __forceinline__ int sched_load(const KvAttnArgs& a, Sched& sc, int64_
 }
 
 template <int D, int CODES, int MT>
-__global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel(const KvAttnArgs a) {
+__global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, 1) kv_attn_rows_kernel(const KvAttnArgs a) {
   using C = RowsCfg<D, MT>;
-  constexpr int TILE = MT * 16, NT = D / 8;
+  constexpr int TILE = MT * 16, NT = D / 8, kWarps = C::kWarps, kThreads = C::kThreads, kUnit = C::kUnit;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ Sched sc;
+  __shared__ Sched<kWarps> sc;
   __shared__ float row_c[TILE];                   // c of the row: scale * log2 e and the power of two taken out of q
-  __shared__ float2 ml[kWarps][TILE];
+  __shared__ float2 ml[kWarps][TILE], ml_all[TILE];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   uint8_t* ring = smem + warp * C::kRing;
   const uint32_t ring_u = smem_u32(ring);
@@ -132,22 +135,25 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
   int64_t all = 0;
   int here = 0;
   for (int64_t base = 0; base < a.slots; base += kThreads) {
-    here = sched_load<TILE>(a, sc, base);
+    here = sched_load<TILE, kWarps>(a, sc, base);
     all += here;
   }
   all *= a.c.kv_heads;
   // no more workers than units: every worker's range then holds a unit, and an item's parts are consecutive workers'
   const int64_t workers = all < gridDim.x ? all : gridDim.x, w = blockIdx.x;
-  if (w >= workers) return;
+  if (w >= workers) {
+    if (threadIdx.x == 0) a.meta[w] = make_int4(0, 0, 0, 0);
+    return;
+  }
   int64_t x = all * w / workers;
   const int64_t x_end = all * (w + 1) / workers;
   // find x: the slots' units before `base`, then inside the chunk
   int64_t base = 0, before = 0;
-  if (a.slots > kThreads) here = sched_load<TILE>(a, sc, 0);
+  if (a.slots > kThreads) here = sched_load<TILE, kWarps>(a, sc, 0);
   while (x >= (before + here) * a.c.kv_heads) {
     before += here;
     base += kThreads;
-    here = sched_load<TILE>(a, sc, base);
+    here = sched_load<TILE, kWarps>(a, sc, base);
   }
   {
     const int64_t p0 = (before + sc.pre[threadIdx.x]) * a.c.kv_heads;
@@ -155,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
   }
   __syncthreads();
   int li = sc.found;
-  bool first_segment = true;
+  bool first_segment = true, cut = false;
   const int group_log2 = a.c.page_log2 - 4, group_mask = (1 << group_log2) - 1;  // 16-key groups of a page
   const uint32_t pool = (uint32_t)a.c.pages;
   const int64_t page_bytes = (int64_t)a.c.kv_heads * a.c.page * D;
@@ -187,15 +193,14 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
     const float* k_scale = a.c.k_scale + kvh;
     const float* v_scale = a.c.v_scale + kvh;
 
-    // page of step st or of the last one, -1 where the table names none (keys below sl.hi lie within the table's width;
-    // a warp without a step looks at the item's first page)
-    auto page_of = [&](int st) -> int {
+    // table entry of step st or of the last one (keys below sl.hi lie within the table's width; a warp without a step
+    // looks at the item's first page).  It is looked at only where it is used, steps later: the load is not waited for here.
+    auto entry_of = [&](int st) -> int {
       const int grp = steps > 0 ? group0 + min(st, steps - 1) * kWarps : group0 - warp;
-      const int p = __ldg(table + (grp >> group_log2));
-      return (uint32_t)p < pool ? p : -1;
+      return __ldg(table + (grp >> group_log2));
     };
     auto issue = [&](int st, int page, uint32_t dst) {
-      if (page >= 0 && st < steps) {
+      if ((uint32_t)page < pool && st < steps) {
         const int64_t off = page * page_bytes + (int64_t)(((kvh << group_log2) + ((group0 + st * kWarps) & group_mask)) * (16 * D)) + lane * 16;
         const uint8_t* ks = a.c.k + off;
         const uint8_t* vs = a.c.v + off;
@@ -211,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
 
     int pages[C::kStages + 1];  // pages of the steps from the one consumed next on
 #pragma unroll
-    for (int i = 0; i <= C::kStages; ++i) pages[i] = page_of(i);
+    for (int i = 0; i <= C::kStages; ++i) pages[i] = entry_of(i);
     uint32_t cur = ring_u, put = ring_u;
     auto next = [&](uint32_t& x) {
       x += C::kStageBytes;
@@ -222,7 +227,9 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
       issue(i, pages[i], put);
       next(put);
     }
-    auto scale_of = [&](const float* s, int page) { return __ldg(s + (int64_t)max(page, 0) * a.c.kv_heads); };
+    auto scale_of = [&](const float* s, int page) {
+      return __ldg(s + (int64_t)((uint32_t)page < pool ? page : 0) * a.c.kv_heads);
+    };
     float ks_next = scale_of(k_scale, pages[0]), vs_next = scale_of(v_scale, pages[0]);
 
     // ---------------------------------------------------------------- q: f16 in the order of the A fragments
@@ -304,12 +311,12 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
       const float ks = ks_next, vs = fmaxf(vs_next, kKvScaleFloor);
 #pragma unroll
       for (int i = 0; i < C::kStages; ++i) pages[i] = pages[i + 1];
-      pages[C::kStages] = page_of(st + C::kStages + 1);
+      pages[C::kStages] = entry_of(st + C::kStages + 1);
       ks_next = scale_of(k_scale, pages[0]);
       vs_next = scale_of(v_scale, pages[0]);
       const uint32_t kt = cur, vt = cur + 16 * D;
       next(cur);
-      if (page < 0) continue;
+      if ((uint32_t)page >= pool) continue;
 
       // ------------------------------------------------------------ S = Q K^T: two 8-key tiles
       float s[MT][2][4];
@@ -487,21 +494,24 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
                          : "memory");
           }
       }
+    if (threadIdx.x < TILE) {
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) m = fmaxf(m, ml[k][threadIdx.x].x);
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const float2 e = ml[k][threadIdx.x];
+        l += e.x == -INFINITY ? 0.f : e.y * kv_ex2(e.x - m);
+      }
+      ml_all[threadIdx.x] = make_float2(m, l);
+    }
     __syncthreads();
     const int part_slot = (int)(w * 2 + (first_segment ? 0 : 1));
     float* part = a.part + (int64_t)part_slot * TILE * (D + 2);
-    for (int i = threadIdx.x; i < TILE * (D / 4); i += kThreads) {
+    for (int i = threadIdx.x; i < sl.rows * (D / 4); i += kThreads) {
       const int r = i / (D / 4), ch = i % (D / 4), tt = ch / (D / 16);
-      if (r >= sl.rows) continue;
       const uint32_t o = (uint32_t)(r * D * 4 + ((ch ^ ((tt * 2 + (r & 1)) & 7)) << 4));
-      float m = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) m = fmaxf(m, ml[k][r].x);
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        const float2 e = ml[k][r];
-        l += e.x == -INFINITY ? 0.f : e.y * kv_ex2(e.x - m);
-      }
+      const float2 e = ml_all[r];
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < kWarps; ++k) {
@@ -512,27 +522,25 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
         sum.w += v.w;
       }
       if (whole) {
-        const int64_t ro = kv_row_out(a, sl, kvh, r);
-        const float inv = l > 0.f ? __fdiv_rn(1.f, l) : (l == 0.f ? 0.f : l);  // a NaN goes through
-        uint2 o2;
-        o2.x = kv_pack(sum.x * inv, sum.y * inv, a.kind);
-        o2.y = kv_pack(sum.z * inv, sum.w * inv, a.kind);
-        *reinterpret_cast<uint2*>(a.out + ro * D + ch * 4) = o2;
-        if (a.lse && ch == 0) a.lse[ro] = l == 0.f ? -INFINITY : 0.6931471805599453f * (m + log2f(l));
+        kv_put_row(a, kv_row_out(a, sl, kvh, r), ch, D, sum, e.x, e.y);
       } else {
         *reinterpret_cast<float4*>(part + (int64_t)r * D + ch * 4) = sum;
-        if (ch == 0) *reinterpret_cast<float2*>(part + (int64_t)TILE * D + 2 * r) = make_float2(m, l);
+        if (ch == 0) *reinterpret_cast<float2*>(part + (int64_t)TILE * D + 2 * r) = e;
       }
     }
-    if (u0 == 0 && threadIdx.x == 0) {
+    if (u0 == 0 && !whole && threadIdx.x == 0) {
       // who holds the rest: the worker of unit y is the last one whose range begins at or before y
       const int64_t y = item0 + (int64_t)kvh * units + units - 1;
       const int64_t w1 = ((y + 1) * workers - 1) / all;
-      a.meta[(base + li) * a.c.kv_heads + kvh] = make_int4(part_slot, (int)(w1 - w) + 1, (int)w, 0);
+      a.meta[w] = make_int4((int)(base + li), kvh, part_slot, (int)(w1 - w) + 1);
+      cut = true;
     }
     first_segment = false;
     x += u1 - u0;
-    if (x >= x_end) break;
+    if (x >= x_end) {
+      if (threadIdx.x == 0 && !cut) a.meta[w] = make_int4(0, 0, 0, 0);
+      break;
+    }
     __syncthreads();  // the rings, q and the statistics are read: the next segment may fill them
     if (x >= item0 + (int64_t)units * a.c.kv_heads) {  // the next slot that has units
       ++li;
@@ -541,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
         if (li < kThreads) break;
         before += here;
         base += kThreads;
-        here = sched_load<TILE>(a, sc, base);
+        here = sched_load<TILE, kWarps>(a, sc, base);
         li = 0;
       }
     }
@@ -550,49 +558,108 @@ __global__ void __launch_bounds__(kThreads, MT == 1 ? 2 : 1) kv_attn_rows_kernel
 
 }  // namespace
 
-// Joins the parts of the items that were cut, in their order, and writes the rows of slots without keys: a warp a row.
+// Block (w, y) of the first a.workers: rows of the item that worker w began and others went on with (at most one).  A
+// thread takes four columns of a row and adds the parts in their order, each with its factor 2^(m_i - m).  The blocks
+// after them look through the slots for those without any key, whose rows are zeros, and for sequences that no kernel of
+// the call takes, whose rows are NaN.
 template <int D, int TILE>
 __global__ void __launch_bounds__(256) kv_attn_join_kernel(const KvAttnArgs a) {
-  constexpr int E = D / 32;
-  const int64_t item = blockIdx.x;
-  const int64_t slot = item / a.c.kv_heads;
-  const int kvh = (int)(item % a.c.kv_heads);
+  constexpr int CH = D / 4, ROWS = 256 / CH;  // 16-byte chunks of a row, rows of a block
+  __shared__ float factor[ROWS][kMaxWorkers];
+  __shared__ float2 ml[ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if ((int)blockIdx.x >= a.workers) {
+    if (blockIdx.y > 0) return;
+    const int64_t slot0 = ((int64_t)(blockIdx.x - a.workers) * 8 + warp) * 32;
+    KvSlot t;
+    bool none = false, over = false;
+    if (slot0 + lane < a.slots) {
+      const int b = a.one ? (int)(slot0 + lane) : kv_slot_seq(a.s, slot0 + lane, a.per, TILE, 1);
+      none = kv_slot(a, slot0 + lane, b, TILE, t) && t.hi <= t.lo;
+      if (a.last) {  // a sequence of more new tokens than the caller allowed for
+        t.s0 = kv_start(a.s, b);
+        const int64_t all = (int64_t)(kv_start(a.s, b + 1) - t.s0) * a.per;
+        over = all > a.row_hi;
+        if (over) {
+          t.r0 = 0;
+          t.rows = (int)all;
+        }
+      }
+    }
+    unsigned todo = __ballot_sync(0xffffffffu, none || over);
+    const unsigned bad = __ballot_sync(0xffffffffu, over);
+    while (todo) {
+      const int src = __ffs(todo) - 1;
+      todo &= todo - 1;
+      KvSlot e;
+      e.s0 = __shfl_sync(0xffffffffu, t.s0, src);
+      e.r0 = __shfl_sync(0xffffffffu, t.r0, src);
+      const int rows = __shfl_sync(0xffffffffu, t.rows, src);
+      const float l = bad >> src & 1 ? __int_as_float(0x7fffffff) : 0.f;
+      for (int64_t i = lane; i < (int64_t)rows * a.c.kv_heads * CH; i += 32) {
+        const int64_t row = i / CH;
+        kv_put_row(a, kv_row_out(a, e, (int)(row / rows), (int)(row % rows)), (int)(i % CH), D, make_float4(0.f, 0.f, 0.f, 0.f),
+                   0.f, l);
+      }
+    }
+    return;
+  }
+  const int4 meta = a.meta[blockIdx.x];
+  // no cut item; or the worker gave up (a time-out, latched in the error word) before it wrote its entry
+  if (meta.w <= 1 || meta.w > a.workers - (int)blockIdx.x || meta.x < 0 || meta.x >= a.slots || meta.y < 0 ||
+      meta.y >= a.c.kv_heads || (meta.z >> 1) != (int)blockIdx.x)
+    return;
+  const int64_t slot = meta.x;
+  const int kvh = meta.y, n = meta.w;
   const int b = a.one ? (int)slot : kv_slot_seq_warp(a.s, slot, a.per, TILE, 1);
   KvSlot sl;
-  if (!kv_slot(a, slot, b, TILE, sl)) return;
-  const bool none = sl.hi <= sl.lo;
-  int4 meta = make_int4(0, 0, 0, 0);
-  if (!none) {
-    meta = a.meta[item];
-    if (meta.y <= 1) return;  // written whole
-  }
-  for (int r = warp; r < sl.rows; r += 8) {
-    float m = -INFINITY, l = 0.f, o[E];
+  const int row0 = blockIdx.y * ROWS;
+  if (!kv_slot(a, slot, b, TILE, sl) || row0 >= sl.rows) return;
+  // the first part is in the slot that its worker says, the others are their worker's first segment
+  auto part_of = [&](int i) { return a.part + (int64_t)(i == 0 ? meta.z : 2 * ((int)blockIdx.x + i)) * TILE * (D + 2); };
+  for (int r = warp; r < ROWS; r += 8) {
+    float m = -INFINITY, l = 0.f;
+    if (row0 + r < sl.rows) {
+      for (int i = lane; i < n; i += 32) {
+        const float x = part_of(i)[(int64_t)TILE * D + 2 * (row0 + r)];
+        factor[r][i] = x;
+        m = fmaxf(m, x);
+      }
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-    for (int i = 0; i < meta.y; ++i) {  // later parts are their worker's first segment
-      const float* part = a.part + (int64_t)(i == 0 ? meta.x : 2 * (meta.z + i)) * TILE * (D + 2);
-      const float2 e2 = *reinterpret_cast<const float2*>(part + (int64_t)TILE * D + 2 * r);
-      if (e2.x == -INFINITY) continue;
-      const float mn = fmaxf(m, e2.x);
-      const float f = m == -INFINITY ? 0.f : kv_ex2(m - mn), f2 = kv_ex2(e2.x - mn);
-      l = l * f + e2.y * f2;
+      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      for (int i = lane; i < n; i += 32) {
+        const float f = factor[r][i] == -INFINITY ? 0.f : kv_ex2(factor[r][i] - m);
+        factor[r][i] = f;
+        l = __fmaf_rn(f, part_of(i)[(int64_t)TILE * D + 2 * (row0 + r) + 1], l);
+      }
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = o[e] * f + part[(int64_t)r * D + lane * E + e] * f2;
-      m = mn;
+      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     }
-    const int64_t ro = kv_row_out(a, sl, kvh, r);
-    const float inv = l > 0.f ? __fdiv_rn(1.f, l) : (l == 0.f ? 0.f : l);
-    uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + ro * D + lane * E);
-#pragma unroll
-    for (int e = 0; e < E / 2; ++e) dst[e] = kv_pack(o[2 * e] * inv, o[2 * e + 1] * inv, a.kind);
-    if (a.lse && lane == 0) a.lse[ro] = l == 0.f ? -INFINITY : 0.6931471805599453f * (m + log2f(l));
+    if (lane == 0) ml[r] = make_float2(m, l);
   }
+  __syncthreads();
+  // neighbours in a warp are rows where the parts are [chunk][row] (tiles of 256), chunks where they are [row][chunk]
+  const int r = TILE == 256 ? threadIdx.x % ROWS : threadIdx.x / CH, ch = TILE == 256 ? threadIdx.x / ROWS : threadIdx.x % CH;
+  if (row0 + r >= sl.rows) return;
+  const int64_t at = TILE == 256 ? ((int64_t)ch * TILE + row0 + r) * 4 : (int64_t)(row0 + r) * D + ch * 4;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float f = factor[r][i];
+    const float4 v = *reinterpret_cast<const float4*>(part_of(i) + at);
+    if (f > 0.f) {  // a part that saw no key of the row may hold anything
+      o.x = __fmaf_rn(v.x, f, o.x);
+      o.y = __fmaf_rn(v.y, f, o.y);
+      o.z = __fmaf_rn(v.z, f, o.z);
+      o.w = __fmaf_rn(v.w, f, o.w);
+    }
+  }
+  kv_put_row(a, kv_row_out(a, sl, kvh, row0 + r), ch, D, o, ml[r].x, ml[r].y);
 }
 
 cudaError_t launch_kv_attn_join(const KvAttnArgs& a, int tile, cudaStream_t st) {
-  const unsigned grid = (unsigned)(a.slots * a.c.kv_heads);
+  if (a.workers > kMaxWorkers) return cudaErrorInvalidValue;
+  const dim3 grid((unsigned)(a.workers + (a.slots + 255) / 256), (unsigned)(tile / (1024 / a.c.dim)));
 #define H3Q_KV_J(DD, TT)                                     \
   if (a.c.dim == DD && tile == TT) {                         \
     kv_attn_join_kernel<DD, TT><<<grid, 256, 0, st>>>(a);    \
@@ -618,14 +685,15 @@ cudaError_t launch_rows(KvAttnArgs a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     ready[dev] = true;
   }
-  kern<<<(unsigned)(sm_count(dev) * (MT == 1 ? 2 : 1)), kThreads, C::kSmem, st>>>(a);
+  a.workers = sm_count(dev);
+  kern<<<(unsigned)a.workers, C::kThreads, C::kSmem, st>>>(a);
   if (const cudaError_t e = cudaGetLastError()) return e;
   return launch_kv_attn_join(a, MT * 16, st);
 }
 
 }  // namespace
 
-size_t kv_attn_rows_part_bytes(int dim, int tile) { return (size_t)sm_count(0) * 4 * tile * (dim + 2) * 4; }
+size_t kv_attn_rows_part_bytes(int dim, int tile) { return (size_t)kMaxWorkers * 2 * tile * (dim + 2) * 4; }
 
 // tile: 16 or 32 rows
 cudaError_t launch_kv_attn_rows(const KvAttnArgs& a, int tile, cudaStream_t st) {

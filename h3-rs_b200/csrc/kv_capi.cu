@@ -125,12 +125,12 @@ AttnPlan plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, in
   if (p.tile) {
     p.slots = batch;
     p.part = a256(kv_attn_rows_part_bytes(dim, p.tile));
-    p.meta = a256((size_t)p.slots * (size_t)kv_heads * sizeof(int4));
+    p.meta = a256(kMaxWorkers * sizeof(int4));
   }
   if (p.chunk) {
     p.chunk_slots = tokens * per / 256 + batch;
     p.chunk_part = a256(kv_attn_chunk_part_bytes(dim));
-    p.chunk_meta = a256((size_t)p.chunk_slots * (size_t)kv_heads * sizeof(int4));
+    p.chunk_meta = a256(kMaxWorkers * sizeof(int4));
     p.chunk_list = a256(kv_attn_chunk_list_bytes(p.chunk_slots));
   }
   p.bytes = p.part + p.meta + p.chunk_part + p.chunk_meta + p.chunk_list;
@@ -259,6 +259,7 @@ h3q_status h3q_kv_attention(const h3q_kv_cache* cache, const void* q, int kind, 
   if (!p.tile) return H3Q_OK;
   a.row_lo = 0;
   a.row_hi = p.tile;
+  a.last = !p.chunk;
   a.one = 1;
   a.slots = p.slots;
   a.part = reinterpret_cast<float*>(ws);

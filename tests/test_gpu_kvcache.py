@@ -246,6 +246,21 @@ def test_attention_without_some_pages(cuda, news):
     assert (got == 0).all() and (lse == -math.inf).all()
 
 
+def test_attention_of_more_tokens_than_allowed_for(cuda):
+    """A sequence that breaks the caller's max_new gets NaN, the others their results; a bound that is not tight changes nothing."""
+    totals, news = [50, 80, 30], [1, 40, 2]
+    cache, table = make_cache(cuda, I8, 2, 16, 64, totals, 6)
+    q = torch.randn((43, 4, 64), generator=_gen(5, cuda), device=cuda).to(BF)
+    args = (q, cache, table, _i32(totals, cuda), _i32(_starts(news), cuda))
+    good, lse = kvcache.attention(*args, max_new=40, return_lse=True)
+    check_attention(q, cache, table, totals, news, good, lse, 0.125, True, 0)
+    assert torch.equal(good, kvcache.attention(*args)) and torch.equal(good, kvcache.attention(*args, max_new=43))
+    got, lse = kvcache.attention(*args, max_new=2, return_lse=True)
+    assert torch.isnan(got[1:41]).all() and torch.isnan(lse[1:41]).all()
+    check_attention(q[:1], cache, table, [50], [1], got[:1], lse[:1], 0.125, True, 0)
+    check_attention(q[41:], cache, table[2:], [30], [2], got[41:], lse[41:], 0.125, True, 0)
+
+
 def test_attention_beyond_32_bit_offsets(cuda):
     """Pages whose codes lie more than 2^32 bytes into the pool."""
     page, hk, dim = 64, 8, 128
