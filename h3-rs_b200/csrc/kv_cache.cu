@@ -23,40 +23,60 @@ struct KvRows {  // rows [tokens, heads, dim] with unit stride inside a head
   int64_t token_stride, head_stride;
 };
 
-// 8 elements of kind KIND as f32; `vec`: 16-byte loads are aligned
+// 8 elements of kind KIND as they lie in memory, and as f32
 template <int KIND>
-__device__ __forceinline__ void load8(const void* base, int64_t off, bool vec, float (&f)[8]) {
+struct Raw8 {
+  uint32_t w[KIND == 0 ? 8 : 4];
+};
+template <int KIND>
+__device__ __forceinline__ void load8(const void* base, int64_t off, bool vec, Raw8<KIND>& r) {
   if (KIND == 0) {
-    const float* p = reinterpret_cast<const float*>(base) + off;
-    if (vec) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-      f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(base) + off;
+    if (vec) {  // 16-byte loads are aligned
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(p)), b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+      r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
+      r.w[KIND == 0 ? 4 : 0] = b.x; r.w[KIND == 0 ? 5 : 0] = b.y; r.w[KIND == 0 ? 6 : 0] = b.z; r.w[KIND == 0 ? 7 : 0] = b.w;
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = __ldg(p + i);
+      for (int i = 0; i < (KIND == 0 ? 8 : 4); ++i) r.w[i] = __ldg(p + i);
     }
   } else {
     const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + off;
-    uint32_t w[4];
     if (vec) {
       const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+      r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldg(p + 2 * i) | ((uint32_t)__ldg(p + 2 * i + 1) << 16);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = KIND == 1 ? h2f((uint16_t)w[i]) : __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = KIND == 1 ? h2f((uint16_t)(w[i] >> 16)) : __uint_as_float(w[i] & 0xffff0000u);
+      for (int i = 0; i < 4; ++i) r.w[i] = (uint32_t)__ldg(p + 2 * i) | ((uint32_t)__ldg(p + 2 * i + 1) << 16);
     }
   }
 }
-
+template <int KIND>
+__device__ __forceinline__ void as_float8(const Raw8<KIND>& r, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (KIND == 0) {
+      f[2 * i] = __uint_as_float(r.w[KIND == 0 ? 2 * i : 0]);
+      f[2 * i + 1] = __uint_as_float(r.w[KIND == 0 ? 2 * i + 1 : 0]);
+    } else {
+      f[2 * i] = KIND == 1 ? h2f((uint16_t)r.w[i]) : __uint_as_float(r.w[i] << 16);
+      f[2 * i + 1] = KIND == 1 ? h2f((uint16_t)(r.w[i] >> 16)) : __uint_as_float(r.w[i] & 0xffff0000u);
+    }
+  }
+}
 __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
   return a <= 3.402823466e38f ? a : 0.f;  // NaN and infinity compare false
+}
+
+// the largest finite magnitude
+template <int KIND>
+__device__ __forceinline__ float amax8(const Raw8<KIND>& r) {
+  float f[8], m = 0.f;
+  as_float8<KIND>(r, f);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(f[e]));
+  return m;
 }
 
 template <int CODES>
@@ -101,8 +121,7 @@ __device__ __forceinline__ bool write_page(const KvCache& c, const KvSeqs& s, co
   const int64_t i = (had >> c.page_log2) + (slot - kv_slot_base(s, b, 1, c.page, 2));
   const int64_t p0 = i << c.page_log2;
   if (p0 >= had + n) return false;
-  w.page = kv_page(c, s, b, i);
-  if (w.page < 0) return false;
+  w.page = kv_page(c, s, b, i);  // -1: the page is not there; its tokens are dropped
   w.lo = had > p0 ? (int)(had - p0) : 0;
   w.hi = had + n - p0 < c.page ? (int)(had + n - p0) : c.page;
   w.token0 = s0 + p0 - had;
@@ -122,63 +141,81 @@ __device__ __forceinline__ uint2 requant8(uint2 w, float ratio) {
                                    __fmul_rn(g[3], ratio)));
 }
 
-// One CTA for a page of a head of K or V: the page's new rows stay in registers between the maximum and the codes, so
-// the input is read once.  VPT vectors of 8 elements a thread: THREADS * VPT * 8 = page * dim.
+template <int KIND, int CODES>
+__device__ __forceinline__ uint2 encode8(const Raw8<KIND>& r, float inv) {
+  float f[8];
+  as_float8<KIND>(r, f);
+  return make_uint2(encode4<CODES>(__fmul_rn(f[0], inv), __fmul_rn(f[1], inv), __fmul_rn(f[2], inv), __fmul_rn(f[3], inv)),
+                    encode4<CODES>(__fmul_rn(f[4], inv), __fmul_rn(f[5], inv), __fmul_rn(f[6], inv), __fmul_rn(f[7], inv)));
+}
+
+// One CTA for a page of K or V and a group of heads, one head after the other: a head's new rows stay in registers
+// between the maximum and the codes, so the input is read once, and the next head's rows are on their way meanwhile.
+// VPT vectors of 8 elements a thread: THREADS * VPT * 8 = page * dim.
 template <int KIND, int CODES, int THREADS, int VPT>
-__global__ void __launch_bounds__(THREADS)
-    kv_write_kernel(KvCache c, KvSeqs s, const int32_t* __restrict__ past, KvRows kr, KvRows vr, int vec) {
+__global__ void __launch_bounds__(THREADS, KIND == 0 ? 768 / THREADS : 1024 / THREADS)
+    kv_write_kernel(KvCache c, KvSeqs s, const int32_t* __restrict__ past, KvRows kr, KvRows vr, int vec, int heads_each) {
   const int64_t slot = blockIdx.x;
-  const int h = blockIdx.y;
   const int b = kv_slot_seq_warp(s, slot, 1, c.page, 2);
   WritePage w;
   if (!write_page(c, s, past, slot, b, w)) return;
   const KvRows r = blockIdx.z ? vr : kr;
-  const int64_t ph = w.page * c.kv_heads + h;
-  float* scale = (blockIdx.z ? c.v_scale : c.k_scale) + ph;
-  uint2* codes = reinterpret_cast<uint2*>((blockIdx.z ? c.v : c.k) + ph * c.page * c.dim);
-  const float old = w.lo > 0 ? *scale : 0.f;
-  const int per_row = c.dim >> 3;
-  float x[VPT][8];
-  float m = 0.f;
+  const int h0 = blockIdx.y * heads_each, h1 = min(c.kv_heads, h0 + heads_each);
+  const int row_log2 = c.dim == 64 ? 3 : 4;  // vectors of a row
+  const bool held = w.lo > 0;
+  // vector j of the thread: row (threadIdx.x + j * THREADS) >> row_log2 of the page
+  const int row0 = threadIdx.x >> row_log2, row_step = THREADS >> row_log2;
+  const int64_t first = (w.token0 + row0) * r.token_stride + (threadIdx.x & ((1 << row_log2) - 1)) * 8;
+  Raw8<KIND> x[VPT], y[VPT];
+  auto is_new = [&](int j) { return row0 + j * row_step >= w.lo && row0 + j * row_step < w.hi; };
+  auto load = [&](int h, Raw8<KIND>(&d)[VPT]) {
+    const int64_t at = first + h * r.head_stride;
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int i = threadIdx.x + j * THREADS, row = i / per_row, col = (i % per_row) * 8;
-    if (row >= w.lo && row < w.hi) {
-      load8<KIND>(r.p, (w.token0 + row) * r.token_stride + h * r.head_stride + col, vec, x[j]);
-    } else {
+    for (int j = 0; j < VPT; ++j) {
+      if (is_new(j)) {
+        load8<KIND>(r.p, at + j * row_step * r.token_stride, vec, d[j]);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[j][e] = 0.f;
+        for (int e = 0; e < (KIND == 0 ? 8 : 4); ++e) d[j].w[e] = 0;
+      }
     }
-  }
-#pragma unroll
-  for (int j = 0; j < VPT; ++j)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(x[j][e]));
-  __shared__ float part[THREADS / 32];
-#pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < THREADS / 32; ++i) m = fmaxf(m, part[i]);
-  const float now = fmaxf(old, fmaxf(__fmul_rn(m, 1.f / top_of(CODES)), kKvScaleFloor));
-  const float inv = __fdiv_rn(1.f, now);
-#pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int i = threadIdx.x + j * THREADS, row = i / per_row;
-    if (row >= w.lo && row < w.hi) {
-      uint2 o;
-      o.x = encode4<CODES>(__fmul_rn(x[j][0], inv), __fmul_rn(x[j][1], inv), __fmul_rn(x[j][2], inv),
-                           __fmul_rn(x[j][3], inv));
-      o.y = encode4<CODES>(__fmul_rn(x[j][4], inv), __fmul_rn(x[j][5], inv), __fmul_rn(x[j][6], inv),
-                           __fmul_rn(x[j][7], inv));
-      codes[i] = o;
-    } else if (row < w.lo && now > old) {
-      codes[i] = requant8<CODES>(codes[i], __fdiv_rn(old, now));
+  };
+  load(h0, x);
+  if (w.page < 0) return;
+  float* scale = (blockIdx.z ? c.v_scale : c.k_scale) + w.page * c.kv_heads;
+  uint2* codes = reinterpret_cast<uint2*>((blockIdx.z ? c.v : c.k) + w.page * c.kv_heads * c.page * c.dim);
+  __shared__ float part[2][THREADS / 32];
+  float old = held ? scale[h0] : 0.f;
+  for (int h = h0; h < h1; ++h) {
+    const bool more = h + 1 < h1;
+    float old_next = 0.f;
+    if (more) {
+      load(h + 1, y);
+      old_next = held ? scale[h + 1] : 0.f;
     }
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) m = fmaxf(m, amax8<KIND>(x[j]));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) part[h & 1][threadIdx.x >> 5] = m;
+    __syncthreads();  // one a head: the other half of `part` is not written before every thread has passed the next one
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) m = fmaxf(m, part[h & 1][i]);
+    const float now = fmaxf(old, fmaxf(__fmul_rn(m, 1.f / top_of(CODES)), kKvScaleFloor));
+    const float inv = __fdiv_rn(1.f, now);
+    uint2* dst = codes + (int64_t)h * (THREADS * VPT);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int i = threadIdx.x + j * THREADS;
+      if (is_new(j)) dst[i] = encode8<KIND, CODES>(x[j], inv);
+      else if (row0 + j * row_step < w.lo && now > old) dst[i] = requant8<CODES>(dst[i], __fdiv_rn(old, now));
+    }
+    if (threadIdx.x == 0) scale[h] = now;  // every thread has read the old scale of head h a head ago
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) x[j] = y[j];
+    old = old_next;
   }
-  // every thread has read the old scale before the barrier above
-  if (threadIdx.x == 0) *scale = now;
 }
 
 // One warp for a page of a head of K or V, for calls of a few tokens a sequence, where a CTA a page would idle: two
@@ -186,40 +223,43 @@ __global__ void __launch_bounds__(THREADS)
 template <int KIND, int CODES>
 __global__ void __launch_bounds__(128)
     kv_write_few_kernel(KvCache c, KvSeqs s, const int32_t* __restrict__ past, KvRows kr, KvRows vr, int vec,
-                        int64_t slots) {
+                        uint32_t slots) {
   const int lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int64_t slot = unit / (2 * c.kv_heads);
+  const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 5);
+  const uint32_t slot = unit / (2 * c.kv_heads);
   if (slot >= slots) return;
   const int rest = (int)(unit % (2 * c.kv_heads)), h = rest >> 1, isv = rest & 1;
   const int b = kv_slot_seq_warp(s, slot, 1, c.page, 2);
   WritePage w;
   if (!write_page(c, s, past, slot, b, w)) return;
   const KvRows r = isv ? vr : kr;
+  const int row_log2 = c.dim == 64 ? 3 : 4;  // vectors of a row
+  const int first = w.lo << row_log2, last = w.hi << row_log2;
+  auto load = [&](int i, Raw8<KIND>& x) {
+    load8<KIND>(r.p, (w.token0 + (i >> row_log2)) * r.token_stride + h * r.head_stride + (i & ((1 << row_log2) - 1)) * 8, vec, x);
+  };
+  Raw8<KIND> x;  // the lane's first vector, which is the only one for one or two tokens
+  const bool any = first + lane < last;
+  if (any) load(first + lane, x);
+  if (w.page < 0) return;
   const int64_t ph = w.page * c.kv_heads + h;
   float* scale = (isv ? c.v_scale : c.k_scale) + ph;
   uint2* codes = reinterpret_cast<uint2*>((isv ? c.v : c.k) + ph * c.page * c.dim);
   const float old = w.lo > 0 ? *scale : 0.f;
-  const int per_row = c.dim >> 3;
-  const int first = w.lo * per_row, last = w.hi * per_row;
-  float m = 0.f;
-  for (int i = first + lane; i < last; i += 32) {
-    float x[8];
-    load8<KIND>(r.p, (w.token0 + i / per_row) * r.token_stride + h * r.head_stride + (i % per_row) * 8, vec, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = fmaxf(m, finite_abs(x[e]));
+  float m = any ? amax8<KIND>(x) : 0.f;
+  for (int i = first + lane + 32; i < last; i += 32) {
+    Raw8<KIND> y;
+    load(i, y);
+    m = fmaxf(m, amax8<KIND>(y));
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float now = fmaxf(old, fmaxf(__fmul_rn(m, 1.f / top_of(CODES)), kKvScaleFloor));
   const float inv = __fdiv_rn(1.f, now);
-  for (int i = first + lane; i < last; i += 32) {
-    float x[8];
-    load8<KIND>(r.p, (w.token0 + i / per_row) * r.token_stride + h * r.head_stride + (i % per_row) * 8, vec, x);
-    uint2 o;
-    o.x = encode4<CODES>(__fmul_rn(x[0], inv), __fmul_rn(x[1], inv), __fmul_rn(x[2], inv), __fmul_rn(x[3], inv));
-    o.y = encode4<CODES>(__fmul_rn(x[4], inv), __fmul_rn(x[5], inv), __fmul_rn(x[6], inv), __fmul_rn(x[7], inv));
-    codes[i] = o;
+  if (any) codes[first + lane] = encode8<KIND, CODES>(x, inv);
+  for (int i = first + lane + 32; i < last; i += 32) {
+    load(i, x);
+    codes[i] = encode8<KIND, CODES>(x, inv);
   }
   if (now > old) {
     const float ratio = __fdiv_rn(old, now);
@@ -250,24 +290,27 @@ __global__ void __launch_bounds__(256)
   const uint8_t* codes = blockIdx.z ? c.v : c.k;
   const float* scale = blockIdx.z ? c.v_scale : c.k_scale;
   void* out = blockIdx.z ? v_out : k_out;
-  const int per_row = c.dim >> 4, per_head = (hi - lo) * per_row;
-  const int total = per_head * (h1 - h0);
+  // The codes of the heads of a page follow one another, `page` rows each: vector v of the group is 16 codes of head
+  // h0 + v / vectors_of_a_head, and every division is a shift.
+  const int row_log2 = c.dim == 64 ? 2 : 3, head_log2 = c.page_log2 + row_log2;
+  const uint4* src = reinterpret_cast<const uint4*>(codes + ((page < 0 ? 0 : page) * c.kv_heads + h0) * c.page * c.dim);
+  const float* sc0 = scale + (page < 0 ? 0 : page) * c.kv_heads + h0;
+  const int total = (h1 - h0) << head_log2;
   for (int i0 = threadIdx.x; i0 < total; i0 += 256 * 4) {
     uint4 w[4];
     float sc[4];
     int64_t dst[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int i = i0 + u * 256;
-      const int h = h0 + i / per_head, j = i % per_head, row = lo + j / per_row, col = (j % per_row) * 16;
+      const int i = i0 + u * 256, h = i >> head_log2, row = (i >> row_log2) & (c.page - 1);
       w[u] = make_uint4(0, 0, 0, 0);
       sc[u] = 0.f;
       dst[u] = -1;
-      if (i < total) {
-        dst[u] = ((token0 + row) * c.kv_heads + h) * c.dim + col;
+      if (i < total && row >= lo && row < hi) {
+        dst[u] = ((token0 + row) * c.kv_heads + h0 + h) * c.dim + (i & ((1 << row_log2) - 1)) * 16;
         if (page >= 0) {  // a token without a page reads as zeros
-          w[u] = __ldg(reinterpret_cast<const uint4*>(codes + ((page * c.kv_heads + h) * c.page + row) * c.dim + col));
-          sc[u] = __ldg(scale + page * c.kv_heads + h);
+          w[u] = __ldg(src + i);
+          sc[u] = __ldg(sc0 + h);
         }
       }
     }
@@ -298,22 +341,31 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// heads a CTA takes: all of them where the pages alone fill the GPU (eight CTAs a multiprocessor), fewer where they do not
+int heads_each(const KvCache& c, int64_t slots) {
+  int groups = 1;
+  while (groups < c.kv_heads && slots * 2 * groups < (int64_t)sm_count(0) * 8) ++groups;
+  return (c.kv_heads + groups - 1) / groups;
+}
+
 template <int KIND, int CODES>
 cudaError_t write_variant(const KvCache& c, const KvSeqs& s, const int32_t* past, const KvRows& k, const KvRows& v,
                           int vec, cudaStream_t st) {
   const int64_t slots = (int64_t)s.tokens / c.page + 2 * (int64_t)s.batch;
   if ((int64_t)s.tokens <= 4 * (int64_t)s.batch) {
     const int64_t warps = slots * c.kv_heads * 2;
-    kv_write_few_kernel<KIND, CODES><<<(unsigned)((warps + 3) / 4), 128, 0, st>>>(c, s, past, k, v, vec, slots);
+    if (warps >= (int64_t)1 << 32) return cudaErrorInvalidValue;
+    kv_write_few_kernel<KIND, CODES><<<(unsigned)((warps + 3) / 4), 128, 0, st>>>(c, s, past, k, v, vec, (uint32_t)slots);
     return cudaGetLastError();
   }
-  const dim3 grid((unsigned)slots, (unsigned)c.kv_heads, 2);
+  const int each = heads_each(c, slots);
+  const dim3 grid((unsigned)slots, (unsigned)((c.kv_heads + each - 1) / each), 2);
   switch (c.page * c.dim) {
-    case 1024: kv_write_kernel<KIND, CODES, 128, 1><<<grid, 128, 0, st>>>(c, s, past, k, v, vec); break;
-    case 2048: kv_write_kernel<KIND, CODES, 128, 2><<<grid, 128, 0, st>>>(c, s, past, k, v, vec); break;
-    case 4096: kv_write_kernel<KIND, CODES, 128, 4><<<grid, 128, 0, st>>>(c, s, past, k, v, vec); break;
-    case 8192: kv_write_kernel<KIND, CODES, 256, 4><<<grid, 256, 0, st>>>(c, s, past, k, v, vec); break;
-    case 16384: kv_write_kernel<KIND, CODES, 512, 4><<<grid, 512, 0, st>>>(c, s, past, k, v, vec); break;
+    case 1024: kv_write_kernel<KIND, CODES, 128, 1><<<grid, 128, 0, st>>>(c, s, past, k, v, vec, each); break;
+    case 2048: kv_write_kernel<KIND, CODES, 128, 2><<<grid, 128, 0, st>>>(c, s, past, k, v, vec, each); break;
+    case 4096: kv_write_kernel<KIND, CODES, 128, 4><<<grid, 128, 0, st>>>(c, s, past, k, v, vec, each); break;
+    case 8192: kv_write_kernel<KIND, CODES, 256, 4><<<grid, 256, 0, st>>>(c, s, past, k, v, vec, each); break;
+    case 16384: kv_write_kernel<KIND, CODES, 512, 4><<<grid, 512, 0, st>>>(c, s, past, k, v, vec, each); break;
     default: return cudaErrorInvalidValue;
   }
   return cudaGetLastError();
@@ -335,10 +387,7 @@ cudaError_t launch_kv_write(const KvCache& c, const KvSeqs& s, const int32_t* pa
 cudaError_t launch_kv_read(const KvCache& c, const KvSeqs& s, const int32_t* first, void* k_out, void* v_out, int kind,
                            cudaStream_t st) {
   const int64_t slots = (int64_t)s.tokens / c.page + 2 * (int64_t)s.batch;
-  // a CTA takes the heads of a page in groups: all of them where the pages alone fill the GPU, fewer where they do not
-  int groups = 1;
-  while (groups < c.kv_heads && slots * 2 * groups < (int64_t)sm_count(0) * 8) ++groups;
-  const int each = (c.kv_heads + groups - 1) / groups;
+  const int each = heads_each(c, slots);
   const dim3 grid((unsigned)slots, (unsigned)((c.kv_heads + each - 1) / each), 2);
 #define H3Q_KV_R(K, C)                                                                 \
   if (kind == K && c.codes == C) {                                                     \

@@ -121,7 +121,10 @@ __device__ __forceinline__ uint32_t kv_pack_f16(float lo, float hi) {
   return r;
 }
 __device__ __forceinline__ uint32_t kv_pack(float lo, float hi, int kind) {
-  return kind == 1 ? kv_pack_f16(lo, hi) : pack_bf2(lo, hi);
+  if (kind == 1) return kv_pack_f16(lo, hi);
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 
 }  // namespace h3q

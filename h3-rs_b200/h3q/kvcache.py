@@ -16,100 +16,118 @@ from __future__ import annotations
 import ctypes
 from dataclasses import dataclass
 
-from . import ERR_ARG, KV_E4M3, KV_INT8, H3QError, KvCacheDesc, _kind, _stream, check, lib
+import torch
+
+from . import ERR_ARG, KV_E4M3, KV_INT8, H3QError, KvCacheDesc, check, lib
+
+_KIND = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_CODES = {torch.int8: KV_INT8, torch.float8_e4m3fn: KV_E4M3}
 
 
 @dataclass
 class KVCache:
     """k, v codes [pages, kv_heads, page, head_dim] (int8 or float8_e4m3fn), k_scale, v_scale f32 [pages, kv_heads]."""
-    k: object
-    v: object
-    k_scale: object
-    v_scale: object
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
 
     def __post_init__(self):
-        import torch
-        if self.k.dim() != 4 or self.k.shape != self.v.shape or self.k.dtype != self.v.dtype:
+        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
+        shape, code = k.shape, _CODES.get(k.dtype)
+        if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype:
             raise H3QError(ERR_ARG, "KVCache: k and v are codes [pages, kv_heads, page, head_dim] of one type")
-        if self.k.dtype not in (torch.int8, torch.float8_e4m3fn):
+        if code is None:
             raise H3QError(ERR_ARG, "KVCache: codes are int8 or float8_e4m3fn")
-        for s in (self.k_scale, self.v_scale):
-            if s.dtype != torch.float32 or s.shape != self.k.shape[:2]:
-                raise H3QError(ERR_ARG, "KVCache: scales are f32 [pages, kv_heads]")
-        for t in (self.k, self.v, self.k_scale, self.v_scale):
-            if not t.is_cuda or not t.is_contiguous() or t.device != self.k.device:
-                raise ValueError("h3q: expected contiguous CUDA tensors of one device")
-        pages, heads, page, dim = self.k.shape
-        self.desc = KvCacheDesc(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
-                                pages, heads, page, dim, KV_INT8 if self.k.dtype == torch.int8 else KV_E4M3)
+        if ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.shape != shape[:2] or vs.shape != shape[:2]:
+            raise H3QError(ERR_ARG, "KVCache: scales are f32 [pages, kv_heads]")
+        self.device = k.get_device()  # -1: not a CUDA tensor
+        if self.device < 0 or not (v.get_device() == ks.get_device() == vs.get_device() == self.device) or not (
+                k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+            raise ValueError("h3q: expected contiguous CUDA tensors of one device")
+        pages, self.heads, page, self.dim = shape
+        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, self.heads, page, self.dim,
+                                code)
+        self.ref = ctypes.byref(self.desc)
 
     @classmethod
-    def empty(cls, pages: int, kv_heads: int, page: int = 64, head_dim: int = 128, dtype=None, device=None):
+    def empty(cls, pages: int, kv_heads: int, page: int = 64, head_dim: int = 128, dtype=torch.int8, device=None):
         """A pool without tokens.  A page's codes and scale mean nothing until its first token is written."""
-        import torch
-        dtype = dtype or torch.int8
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         codes = [torch.empty((pages, kv_heads, page, head_dim), dtype=dtype, device=device) for _ in range(2)]
         scales = [torch.zeros((pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)]
         return cls(codes[0], codes[1], scales[0], scales[1])
 
 
-def _ints(name, t, cache, shape):
-    """t as the int32 tensor that a call reads, checked."""
-    import torch
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != cache.k.device or not t.is_contiguous():
-        raise H3QError(ERR_ARG, f"kvcache: {name} is a contiguous int32 tensor {list(shape)} on the cache's device")
+def _stream(cache) -> int:
+    return torch._C._cuda_getCurrentRawStream(cache.device)
+
+
+def _ints(name, t, cache, n):
+    """The address of t, checked to be the int32 [n] that a call reads; None for None."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or t.get_device() != cache.device or not t.is_contiguous():
+        raise H3QError(ERR_ARG, f"kvcache: {name} is a contiguous int32 tensor [{n}] on the cache's device")
     return t.data_ptr()
 
 
+def _table(t, cache):
+    if t.dtype != torch.int32 or t.dim() != 2 or t.get_device() != cache.device or not t.is_contiguous():
+        raise H3QError(ERR_ARG, "kvcache: the page table is a contiguous int32 tensor [batch, pages] on the cache's device")
+    batch, width = t.shape
+    return t.data_ptr(), batch, width
+
+
 def _rows(name, x, cache, heads):
-    """The strides of rows x [tokens, heads, head_dim] whose heads are contiguous."""
-    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != cache.k.shape[3] or x.device != cache.k.device:
-        raise H3QError(ERR_ARG, f"kvcache: {name} is [tokens, {heads}, {cache.k.shape[3]}] on the cache's device")
+    """The token and head strides of rows x [tokens, heads, head_dim]."""
+    shape = x.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != cache.dim or x.get_device() != cache.device:
+        raise H3QError(ERR_ARG, f"kvcache: {name} is [tokens, {heads}, {cache.dim}] on the cache's device")
     ts, hs, es = x.stride()
     if es != 1:
         raise H3QError(ERR_ARG, f"kvcache: {name} needs unit stride inside a head")
     return ts, hs
 
 
-def _table(page_table, cache):
-    if page_table.dim() != 2:
-        raise H3QError(ERR_ARG, "kvcache: the page table is int32 [batch, pages]")
-    batch, width = page_table.shape
-    return _ints("page_table", page_table, cache, (batch, width)), batch, width
+def _kind(dtype) -> int:
+    kind = _KIND.get(dtype)
+    if kind is None:
+        raise H3QError(ERR_ARG, "kvcache: rows are f32, f16 or bf16")
+    return kind
 
 
 def write(cache: KVCache, k, v, page_table, past, starts=None) -> None:
     """Appends k and v [tokens, kv_heads, head_dim] (f32, f16 or bf16; views of a fused projection are fine) behind the
-    past [batch] tokens of each sequence.  A page's scale is max(old, amax * (1 / top)); where it grows, the page's older codes are
-    rounded anew (h3q_kv_write has the formula)."""
-    heads = cache.k.shape[1]
+    past [batch] tokens of each sequence.  A page's scale is max(old, amax * (1 / top)); where it grows, the page's older
+    codes are rounded anew (h3q_kv_write has the formula)."""
     if k.dtype != v.dtype or k.shape != v.shape:
         raise H3QError(ERR_ARG, "kvcache: k and v have one shape and type")
-    kind = _dtype(k.dtype)
-    kt, kh = _rows("k", k, cache, heads)
-    vt, vh = _rows("v", v, cache, heads)
+    kind = _kind(k.dtype)
+    kt, kh = _rows("k", k, cache, cache.heads)
+    vt, vh = _rows("v", v, cache, cache.heads)
     table, batch, width = _table(page_table, cache)
-    pp = _ints("past", past, cache, (batch,))
-    sp = None if starts is None else _ints("starts", starts, cache, (batch + 1,))
-    check(lib().h3q_kv_write(ctypes.byref(cache.desc), k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, kind, k.shape[0], table,
-                             width, pp, sp, batch, _stream(cache.k.device)))
+    pp = _ints("past", past, cache, batch)
+    sp = _ints("starts", starts, cache, batch + 1)
+    st = lib().h3q_kv_write(cache.ref, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, kind, k.shape[0], table, width, pp, sp,
+                            batch, _stream(cache))
+    if st:
+        check(st)
 
 
-def read(cache: KVCache, page_table, starts, total: int, dtype=None, first=None):
+def read(cache: KVCache, page_table, starts, total: int, dtype=torch.bfloat16, first=None):
     """Tokens first[b] (0 without it) and on of each sequence, starts[b + 1] - starts[b] of them, as dense (k, v)
-    [total, kv_heads, head_dim] of `dtype` (bf16 without it)."""
-    import torch
-    dtype = dtype or torch.bfloat16
-    kind = _dtype(dtype)
+    [total, kv_heads, head_dim] of `dtype`."""
+    kind = _kind(dtype)
     table, batch, width = _table(page_table, cache)
-    sp = None if starts is None else _ints("starts", starts, cache, (batch + 1,))
-    fp = None if first is None else _ints("first", first, cache, (batch,))
-    shape = (total, cache.k.shape[1], cache.k.shape[3])
-    k = torch.empty(shape, dtype=dtype, device=cache.k.device)
-    v = torch.empty(shape, dtype=dtype, device=cache.k.device)
-    check(lib().h3q_kv_read(ctypes.byref(cache.desc), table, width, fp, sp, batch, total, k.data_ptr(), v.data_ptr(), kind,
-                            _stream(cache.k.device)))
+    sp = _ints("starts", starts, cache, batch + 1)
+    fp = _ints("first", first, cache, batch)
+    shape = (total, cache.heads, cache.dim)
+    k = cache.k.new_empty(shape, dtype=dtype)
+    v = torch.empty_like(k)
+    st = lib().h3q_kv_read(cache.ref, table, width, fp, sp, batch, total, k.data_ptr(), v.data_ptr(), kind, _stream(cache))
+    if st:
+        check(st)
     return k, v
 
 
@@ -120,33 +138,27 @@ def attention(q, cache: KVCache, page_table, lengths, starts=None, scale: float 
     last `window` keys of each row.  max_new: an upper bound of the new tokens of one sequence, where starts is given and the
     host knows one.  Returns [tokens, heads, head_dim], and with return_lse the f32 [tokens, heads] logarithms of the
     sums of exponentials."""
-    import torch
-    if q.dtype not in (torch.float16, torch.bfloat16):
+    if q.dtype != torch.bfloat16 and q.dtype != torch.float16:
         raise H3QError(ERR_ARG, "kvcache: q is f16 or bf16")
     qt, qh = _rows("q", q, cache, q.shape[1] if q.dim() == 3 else 0)
     tokens, heads, dim = q.shape
     table, batch, width = _table(page_table, cache)
-    lp = _ints("lengths", lengths, cache, (batch,))
-    sp = None if starts is None else _ints("starts", starts, cache, (batch + 1,))
-    out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
-    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    lp = _ints("lengths", lengths, cache, batch)
+    sp = _ints("starts", starts, cache, batch + 1)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     if starts is None and batch:
         max_new = tokens // batch
-    need = lib().h3q_kv_attention_workspace_size(tokens, batch, heads, cache.desc.kv_heads, dim, max_new)
+    L = lib()
+    need = L.h3q_kv_attention_workspace_size(tokens, batch, heads, cache.heads, dim, max_new)
     if workspace is None or workspace.numel() < need:
-        workspace = torch.empty(max(need, 1), dtype=torch.uint8, device=q.device)
-    check(lib().h3q_kv_attention(ctypes.byref(cache.desc), q.data_ptr(), _kind(q.dtype), qt, qh, tokens, heads, table, width,
-                                 lp, sp, batch, max_new, dim ** -0.5 if scale is None else scale, int(causal), window,
-                                 out.data_ptr(), None if lse is None else lse.data_ptr(), workspace.data_ptr(),
-                                 workspace.numel(), _stream(q.device)))
+        workspace = q.new_empty(need, dtype=torch.uint8)
+    st = L.h3q_kv_attention(cache.ref, q.data_ptr(), _KIND[q.dtype], qt, qh, tokens, heads, table, width, lp, sp, batch,
+                            max_new, dim ** -0.5 if scale is None else scale, causal, window, out.data_ptr(),
+                            lse.data_ptr() if return_lse else None, workspace.data_ptr(), workspace.numel(), _stream(cache))
+    if st:
+        check(st)
     return (out, lse) if return_lse else out
-
-
-def _dtype(dtype) -> int:
-    import torch
-    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
-        raise H3QError(ERR_ARG, "kvcache: rows are f32, f16 or bf16")
-    return _kind(dtype)
 
 
 __all__ = ["KVCache", "write", "read", "attention"]
