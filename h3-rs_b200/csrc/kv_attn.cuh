@@ -7,8 +7,8 @@
 // so K and V enter the tensor cores as their codes, which 16-bit floats hold exactly, and one scale a page is applied
 // in f32.  What is rounded is w (f16) and the output; m, l, the scores and O are f32.
 //
-// q enters as f16: an f16 input as it is; a bf16 row times a power of two that brings its largest element into
-// [1, 2), which is exact but for elements below 2^-14 of the row's largest (their error is under 2^-25 of it).
+// q enters as f16: an f16 input as it is; a bf16 row times a power of two that brings its largest element near 1, which
+// is exact but for elements below 2^-14 of the row's largest (their error is under 2^-25 of it).
 #pragma once
 #include "kv_common.cuh"
 
@@ -83,6 +83,18 @@ __device__ __forceinline__ void kv_row_keys(const KvAttnArgs& a, const KvSlot& t
 __device__ __forceinline__ int64_t kv_row_out(const KvAttnArgs& a, const KvSlot& t, int kvh, int r) {
   const int rr = t.r0 + r;
   return (int64_t)(t.s0 + rr / a.per) * a.heads + kvh * a.per + rr % a.per;
+}
+
+// For a bf16 row of largest magnitude mx: f, the power of two that brings it into [1, 4) ([1, 2) but for the last
+// binade, whose inverse is no normal number; a row below the normal range comes out smaller), and c times its inverse.
+__device__ __forceinline__ void kv_row_scale(float mx, float& f, float& c) {
+  f = 1.f;
+  if (mx > 0.f && mx < INFINITY) {
+    int e = (int)(__float_as_uint(mx) >> 23) - 127;
+    e = e < -126 ? -126 : (e > 126 ? 126 : e);
+    f = __uint_as_float((uint32_t)(127 - e) << 23);
+    c *= __uint_as_float((uint32_t)(127 + e) << 23);
+  }
 }
 
 // four columns (chunk ch) of output row ro, from the unnormalised sums and the row's statistics

@@ -9,8 +9,9 @@
 //                over the scores it came from (the A operand of the second product is read from there: with W in
 //                shared memory the products alone would take the SM's whole shared-memory bandwidth), row sums; the
 //                maximum moves only when a tile raises it by more than 2^8;
-//   warp 1       walks the page table ahead of them: the address and the scales of each 16 keys, into a ring in shared
-//                memory, so that the others never wait for a table entry before they can ask for what it names;
+//   warp 1       walks the work ahead of them: which rows and keys come next, and from the page table the address and
+//                the scales of each 16 keys, into rings in shared memory, so that the others never wait for a length
+//                or a table entry before they can ask for what it names;
 //   warps 12-15  widen codes to f16 into a ring of five 128-key tiles, K and V in turn: codes come straight from global memory into registers one tile ahead, K rows go out as
 //                they are, V is transposed on the way (byte permutes between eight keys of a thread), both in the
 //                K-major 128-byte-swizzle layout.
@@ -46,8 +47,9 @@ struct Cfg {
   static constexpr int OFF_KV = NQ * Q_TILE;
   static constexpr int OFF_SC = OFF_KV + RING * KV_TILE;
   static constexpr int OFF_ADDR = OFF_SC + WR * 8 * 16;
-  static constexpr int OFF_BAR = OFF_ADDR + WR * 8 * 8;
-  static constexpr int NBAR = 2 * RING + 2 * WR + 4 * NQ + 1;
+  static constexpr int OFF_SEG = OFF_ADDR + WR * 8 * 8;
+  static constexpr int OFF_BAR = OFF_SEG + 2 * 48;
+  static constexpr int NBAR = 2 * RING + 2 * WR + 4 * NQ + 1 + 4;
   static constexpr size_t SMEM = 1024 + OFF_BAR + NBAR * 8 + 16;
   static_assert(SMEM + 16 <= 232448, "shared memory exceeds the sm_100 per-CTA limit");
 };
@@ -60,6 +62,14 @@ __device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
   return d;
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(p)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 r;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
+  return r;
+}
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -153,7 +163,16 @@ __global__ void __launch_bounds__(1024) kv_attn_list_kernel(const KvAttnArgs a, 
 
 namespace {
 
-// A CTA's walk over its range of tiles: every role steps through the same segments.
+// A stretch of tiles of one item, as the walker hands it to the other roles.
+struct Stretch {
+  int rows, n;          // rows of the slot, tiles (0: the end)
+  int s0, r0, fresh;    // of the slot's sequence: first packed row, first row of the slot, new tokens
+  int kvh, whole, pad;
+  int64_t len, key_base;
+};
+static_assert(sizeof(Stretch) == 48, "two of them in shared memory");
+
+// The walker's place in its CTA's range of tiles.
 struct Walk {
   int64_t x, end;
   int i;  // index into the list
@@ -194,10 +213,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* s_full = q_full + NQ;
   uint64_t* p_full = s_full + NQ;
   uint64_t* o_full = p_full + NQ;
-  uint64_t* mma_done = o_full + NQ;
+  uint64_t* sg_full = o_full + NQ;
+  uint64_t* sg_free = sg_full + 2;
+  uint64_t* mma_done = sg_free + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  __shared__ int first_i;
+  const Stretch* stretches = reinterpret_cast<const Stretch*>(smem + C::OFF_SEG);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t all = wk.head[1], workers = all < gridDim.x ? all : gridDim.x;
@@ -205,7 +226,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (threadIdx.x == 0) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
-  Walk walk{all * blockIdx.x / workers, all * (blockIdx.x + 1) / workers, 0};
   if (threadIdx.x == 0) {
     for (int i = 0; i < RING; ++i) { mbar_init(&kv_full[i], 4); mbar_init(&kv_empty[i], 1); }
     for (int i = 0; i < WR; ++i) { mbar_init(&wr_full[i], 1); mbar_init(&wr_free[i], 4); }
@@ -215,16 +235,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&p_full[t], 4);
       mbar_init(&o_full[t], 1);
     }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sg_full[i], 1);
+      mbar_init(&sg_free[i], 1 + 4 + 8);  // the MMA thread, the decode and the softmax warps
+    }
     mbar_init(mma_done, 1);
     *abort_flag = 0;
     fence_barrier_init();
-    int lo = 0, hi = (int)wk.head[0];  // the last listed slot whose tiles begin at or before x
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (wk.list[mid].before <= walk.x) lo = mid;
-      else hi = mid;
-    }
-    first_i = lo;
   }
   if (warp == 0) {
     tmem_alloc(tmem_slot, TMEM_COLS);
@@ -234,7 +251,22 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  walk.i = first_i;
+  // the i-th stretch by one thread, and by a warp: waits for it, copies it and tells the walker so
+  auto copy = [&](uint32_t i, Stretch& s) {
+    if (!mbar_wait_prompt(&sg_full[i & 1], (i >> 1) & 1, abort_flag, err, kDevTimeoutScale)) return false;
+    s = stretches[i & 1];
+    return s.n > 0;
+  };
+  auto take = [&](uint32_t i, Stretch& s) {
+    if (!copy(i, s)) return false;
+    mbar_arrive(&sg_free[i & 1]);
+    return true;
+  };
+  auto take_warp = [&](uint32_t i, Stretch& s) {
+    if (!__all_sync(0xffffffffu, copy(i, s))) return false;  // every lane has its copy
+    if (lane == 0) mbar_arrive(&sg_free[i & 1]);
+    return true;
+  };
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_MMA));
@@ -284,10 +316,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       constexpr Int<0> t0{};
       constexpr Int<1> t1{};
-      Segment s;
-      while (ok && next_segment(a, wk, walk, s)) {
-        const bool two = s.sl.rows > BM;
-        const int n = s.t1 - s.t0;
+      Stretch s;
+      for (uint32_t si = 0; ok && take(si, s); ++si) {
+        const bool two = s.rows > BM;
+        const int n = s.n;
         if (!(ok = wait_kv() && mbar_wait_prompt(&q_full[0], segs0++ & 1, abort_flag, err, kDevTimeoutFull))) break;
         tc_fence_after();
         issue_qk(t0);
@@ -324,11 +356,46 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_drain(mma_done, 0, err, kDevTimeoutDrain);
     }
     if (warp == 1) {
-      // ------------------------------------------------------------------ table walker: eight lanes, 16 keys each
-      uint32_t tile = 0;
+      // ------------------------------------------------------------------ walker: for tiles, eight lanes of 16 keys each
+      Walk walk{all * blockIdx.x / workers, all * (blockIdx.x + 1) / workers, 0};
+      for (int hi = (int)wk.head[0]; hi - walk.i > 1;) {  // the last listed slot whose tiles begin at or before x
+        const int mid = (walk.i + hi) >> 1;
+        if (wk.list[mid].before <= walk.x) walk.i = mid;
+        else hi = mid;
+      }
+      uint32_t tile = 0, si = 0;
       bool ok = true;
       Segment s;
+      auto hand = [&](int n) {  // stretch si to the others
+        if (si >= 2 && !__all_sync(0xffffffffu, mbar_wait_prompt(&sg_free[si & 1], ((si >> 1) - 1) & 1, abort_flag, err,
+                                                                 kDevTimeoutEmpty)))
+          return false;
+        if (lane == 0) {
+          Stretch& d = reinterpret_cast<Stretch*>(smem + C::OFF_SEG)[si & 1];
+          d.rows = s.sl.rows;
+          d.n = n;
+          d.s0 = s.sl.s0;
+          d.r0 = s.sl.r0;
+          d.fresh = s.sl.n;
+          d.kvh = s.kvh;
+          d.whole = s.t0 == 0 && s.t1 == s.e.tiles;
+          d.len = s.sl.len;
+          d.key_base = s.sl.lo + (int64_t)s.t0 * BN;
+          mbar_arrive(&sg_full[si & 1]);
+        }
+        ++si;
+        return true;
+      };
+      bool cut = false;
       while (ok && next_segment(a, wk, walk, s)) {
+        if (lane == 0 && s.t0 == 0 && s.t1 < s.e.tiles) {  // begun here, and others go on with it
+          const int64_t y = s.e.before + (int64_t)(s.kvh + 1) * s.e.tiles - 1;
+          const int64_t w1 = ((y + 1) * workers - 1) / all;
+          a.meta[blockIdx.x] =
+              make_int4(s.e.slot, s.kvh, (int)blockIdx.x * 2 + (si > 0), (int)(w1 - blockIdx.x) + 1);
+          cut = true;
+        }
+        if (!(ok = hand(s.t1 - s.t0))) break;
         int64_t key = s.sl.lo + (int64_t)s.t0 * BN + lane * 16;
         for (int j = s.t0; j < s.t1; ++j, ++tile, key += BN) {
           const int64_t page = lane < 8 && key < s.sl.hi ? kv_page(a.c, a.s, s.sl.b, key >> a.c.page_log2) : -1;
@@ -337,6 +404,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (page >= 0) {
             const int64_t ph = page * a.c.kv_heads + s.kvh;
             off = (ph * a.c.page + (key & (a.c.page - 1))) * D;
+            // the decode warps ask for these codes three tiles from now, and find them in L2
+            prefetch_l2(a.c.k + off, 16 * D);
+            prefetch_l2(a.c.v + off, 16 * D);
             const float vs = fmaxf(__ldg(a.c.v_scale + ph), kKvScaleFloor);
             c = make_float4(__ldg(a.c.k_scale + ph), kv_lg2(vs), __fdividef(1.f, vs), 0.f);
           }
@@ -356,6 +426,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (lane == 0) mbar_arrive(&wr_full[tile % WR]);
         }
       }
+      if (lane == 0 && !cut) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+      if (ok) hand(0);
     }
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_DEC));
@@ -372,10 +444,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t vbuf[8][VW];
     uint32_t seq = 0, tile0 = 0;
     bool ok = true;
-    Segment s;
-    while (ok && next_segment(a, wk, walk, s)) {
-      const int n = s.t1 - s.t0;
-      const int64_t key_base = s.sl.lo + (int64_t)s.t0 * BN;
+    Stretch s;
+    for (uint32_t si = 0; ok && take_warp(si, s); ++si) {
+      const int n = s.n;
       auto load_k = [&](int j) {
         const uint32_t T = tile0 + j;
         if (!__all_sync(0xffffffffu, mbar_wait_prompt(&wr_full[T % WR], (T / WR) & 1, abort_flag, err, kDevTimeoutScale)))
@@ -391,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       };
       auto load_v = [&](int j) {
         const int64_t off = addr[((tile0 + j) % WR) * 8 + (vo >> 1)];
-        const int64_t left = s.sl.len - (key_base + (int64_t)j * BN + vo * 8);  // what lies behind the last token may be any bits
+        const int64_t left = s.len - (s.key_base + (int64_t)j * BN + vo * 8);  // what lies behind the last token may be any bits
         const uint8_t* src = a.c.v + (off < 0 ? 0 : off + (vo & 1) * 8 * D + vc * (D / 8));
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
@@ -480,84 +551,89 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t qrow = smem_u32(smem + g * C::Q_TILE) + rloc * 128;
     const uint32_t swz = rloc & 7;
     uint32_t done = 0, segs = 0, tile0 = 0;
-    bool ok = true, first = true;
-    Segment s;
-    while (ok && next_segment(a, wk, walk, s)) {
-      const int n = s.t1 - s.t0;
-      const bool whole = s.t0 == 0 && s.t1 == s.e.tiles;
-      const int part_slot = (int)blockIdx.x * 2 + (first ? 0 : 1);
-      first = false;
-      if (g == 0 && rloc == 0) {
-        if (s.t0 == 0 && !whole) {
-          const int64_t y = s.e.before + (int64_t)(s.kvh + 1) * s.e.tiles - 1;
-          const int64_t w1 = ((y + 1) * workers - 1) / all;
-          a.meta[blockIdx.x] = make_int4(s.e.slot, s.kvh, part_slot, (int)(w1 - blockIdx.x) + 1);
-        } else if (walk.x >= walk.end) {  // the last segment, and not one that others go on with
-          a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-        }
-      }
-      if (g * BM >= s.sl.rows) {  // a slot of one tile
+    bool ok = true;
+    Stretch s;
+    for (uint32_t si = 0; ok && take_warp(si, s); ++si) {
+      const int n = s.n;
+      const int part_slot = (int)blockIdx.x * 2 + (si > 0);
+      if (g * BM >= s.rows) {  // a slot of one tile
         tile0 += n;
         continue;
       }
       const int r = g * BM + rloc;
-      const bool in = r < s.sl.rows;
+      const bool in = r < s.rows;
+      const int token = (s.r0 + (in ? r : 0)) / a.per;  // of the sequence's new ones
+      const int64_t ro = (int64_t)(s.s0 + token) * a.heads + s.kvh * a.per + (s.r0 + (in ? r : 0)) % a.per;
       // ------------------------------------------------------------ q as f16, the sign of the scale in it
+      // The last stretch's scores of this tile are read, so its products are done with Q.  A warp's 32 rows come in whole
+      // rows, LPQ lanes each, to their places; then every thread scales its own row there.
       float c = fabsf(a.scale_log2);
       {
-        const int rr = s.sl.r0 + (in ? r : 0);
-        const uint16_t* src =
-            a.q + (int64_t)(s.sl.s0 + rr / a.per) * a.q_ts + (int64_t)(s.kvh * a.per + rr % a.per) * a.q_hs;
-        uint32_t w[D / 2];
-        if (q_vec) {
+        constexpr int LPQ = D / 8;  // 16-byte pieces of a row
+        const uint32_t qtile = smem_u32(smem + g * C::Q_TILE) + quarter * 32 * 128;
+        const int64_t src = (int64_t)(s.s0 + token) * a.q_ts + (int64_t)(s.kvh * a.per + (s.r0 + (in ? r : 0)) % a.per) * a.q_hs;
+        const int ch = lane % LPQ;
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            const uint4 v = in ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+        for (int half = 0; half < 2; ++half) {
+          uint4 v[LPQ / 2];
+#pragma unroll
+          for (int i = 0; i < LPQ / 2; ++i) {
+            const int row = (half * (LPQ / 2) + i) * (32 / LPQ) + lane / LPQ;
+            const int64_t at = __shfl_sync(0xffffffffu, src, row) + ch * 8;
+            const bool there = __shfl_sync(0xffffffffu, (int)in, row);
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (there && q_vec) {
+              v[i] = __ldg(reinterpret_cast<const uint4*>(a.q + at));
+            } else if (there) {
+              uint32_t e[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                e[k] = (uint32_t)__ldg(a.q + at + 2 * k) | ((uint32_t)__ldg(a.q + at + 2 * k + 1) << 16);
+              v[i] = make_uint4(e[0], e[1], e[2], e[3]);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < LPQ / 2; ++i) {
+            const int row = (half * (LPQ / 2) + i) * (32 / LPQ) + lane / LPQ;
+            sts128(qtile + row * 128 + (ch >> 3) * C::Q_SLAB + (((ch & 7) ^ (row & 7)) << 4), v[i].x, v[i].y, v[i].z, v[i].w);
+          }
+        }
+        __syncwarp();
+        const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+        if (a.kind == 2 || sign) {
+          uint32_t w[D / 2];
+#pragma unroll
+          for (int i = 0; i < LPQ; ++i) {
+            const uint4 v = lds128(qrow + (i >> 3) * C::Q_SLAB + (((i & 7) ^ swz) << 4));
             w[4 * i] = v.x;
             w[4 * i + 1] = v.y;
             w[4 * i + 2] = v.z;
             w[4 * i + 3] = v.w;
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < D / 2; ++i)
-            w[i] = in ? (uint32_t)__ldg(src + 2 * i) | ((uint32_t)__ldg(src + 2 * i + 1) << 16) : 0u;
-        }
-        if (a.kind == 2) {
-          float mx = 0.f;
-#pragma unroll
-          for (int i = 0; i < D / 2; ++i)
-            mx = max3f(mx, fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u)));
-          float f = 1.f;
-          if (mx > 0.f && mx < INFINITY) {
-            const int e = ilogbf(mx);
-            // 2^-e in two factors: e reaches 127 and (for bf16 below the normal range) -133
-            f = scalbnf(1.f, -e / 2);
-            c = scalbnf(c, e);
-            const float f2nd = scalbnf(1.f, -e - (-e / 2));
+          if (a.kind == 2) {
+            float mx = 0.f, f;
 #pragma unroll
             for (int i = 0; i < D / 2; ++i)
-              w[i] = kv_pack_f16(__uint_as_float(w[i] << 16) * f * f2nd, __uint_as_float(w[i] & 0xffff0000u) * f * f2nd);
-          } else {
+              mx = max3f(mx, fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u)));
+            kv_row_scale(mx, f, c);
 #pragma unroll
             for (int i = 0; i < D / 2; ++i)
-              w[i] = kv_pack_f16(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+              w[i] = kv_pack_f16(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
           }
-        }
-        const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-        // the last segment's S of this tile is read, so its MMAs are done with Q
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-          sts128(qrow + (i >> 3) * C::Q_SLAB + (((i & 7) ^ swz) << 4), w[4 * i] ^ sign, w[4 * i + 1] ^ sign,
-                 w[4 * i + 2] ^ sign, w[4 * i + 3] ^ sign);
+          for (int i = 0; i < LPQ; ++i)
+            sts128(qrow + (i >> 3) * C::Q_SLAB + (((i & 7) ^ swz) << 4), w[4 * i] ^ sign, w[4 * i + 1] ^ sign,
+                   w[4 * i + 2] ^ sign, w[4 * i + 3] ^ sign);
+        }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[g]);
       }
-      const int64_t ro = in ? kv_row_out(a, s.sl, s.kvh, r) : 0;
-      const int64_t key_base = s.sl.lo + (int64_t)s.t0 * BN;
-      int64_t lo = 0, hi = s.sl.hi;
-      if (in) kv_row_keys(a, s.sl, r, lo, hi);  // a row that is not there sees all: its warp is spared the mask
+      // the keys of the row; a row that is not there sees all: its warp is spared the mask
+      const int64_t pos = s.len - s.fresh + token;
+      const int64_t key_base = s.key_base;
+      const int64_t hi = in && a.causal && pos + 1 < s.len ? pos + 1 : s.len;
+      const int64_t lo = in && a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0;
       const int64_t span = (int64_t)n * BN;
       const int klo = (int)(lo < key_base ? 0 : (lo - key_base < span ? lo - key_base : span));
       const int khi = (int)(hi < key_base ? 0 : (hi - key_base < span ? hi - key_base : span));
@@ -667,25 +743,38 @@ __global__ void __launch_bounds__(THREADS, 1)
         uint32_t o[32];
         tmem_ld_32x32b_x32(tO + 32 * k, o);
         tmem_wait_ld();
-        if (!in) continue;
-        if (whole) {
-          uint4* d4 = reinterpret_cast<uint4*>(a.out + ro * D + 32 * k);
+        if (s.whole) {  // 16-bit rows, through the tile's Q (its products are done), so that whole rows go out
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               w[e] = kv_pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv, a.kind);
-            d4[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            const int ch = 4 * k + i;
+            sts128(qrow + (ch >> 3) * C::Q_SLAB + (((ch & 7) ^ swz) << 4), w[0], w[1], w[2], w[3]);
           }
-        } else {
+        } else if (in) {
           uint4* d4 = reinterpret_cast<uint4*>(part) + (int64_t)(8 * k) * ROWS + r;  // a warp's rows are neighbours
 #pragma unroll
           for (int i = 0; i < 8; ++i) d4[i * ROWS] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
       }
+      if (s.whole) {
+        __syncwarp();
+        constexpr int LPQ = D / 8;
+        const uint32_t qtile = smem_u32(smem + g * C::Q_TILE) + quarter * 32 * 128;
+        const int ch = lane % LPQ;
+#pragma unroll 4
+        for (int i = 0; i < LPQ; ++i) {
+          const int row = i * (32 / LPQ) + lane / LPQ;
+          const uint4 v = lds128(qtile + row * 128 + (ch >> 3) * C::Q_SLAB + (((ch & 7) ^ (row & 7)) << 4));
+          const int64_t to = __shfl_sync(0xffffffffu, ro, row);
+          if (__shfl_sync(0xffffffffu, (int)in, row)) *reinterpret_cast<uint4*>(a.out + to * D + ch * 8) = v;
+        }
+        __syncwarp();  // read before the next stretch's rows go there
+      }
       if (in) {
-        if (!whole) *reinterpret_cast<float2*>(part + (int64_t)ROWS * D + 2 * r) = make_float2(m_used, l);
+        if (!s.whole) *reinterpret_cast<float2*>(part + (int64_t)ROWS * D + 2 * r) = make_float2(m_used, l);
         else if (a.lse) a.lse[ro] = l == 0.f ? -INFINITY : 0.6931471805599453f * (m_used + log2f(l));
       }
       tc_fence_before();  // the reads of O are ordered before the next segment's first product, through p_full

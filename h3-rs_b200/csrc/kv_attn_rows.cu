@@ -250,12 +250,10 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, 1) kv_attn_rows_kern
       if (a.kind == 2) {
 #pragma unroll
         for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        if (mx > 0.f && mx < INFINITY) {
-          const int e = ilogbf(mx);
+        float p2;
+        kv_row_scale(mx, p2, c);
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) f[i] = scalbnf(f[i], -e);
-          c = scalbnf(c, e);
-        }
+        for (int i = 0; i < D / 32; ++i) f[i] *= p2;
       }
       if (lane == 0) row_c[r] = c;
       // element d of the row: lane t = d / (D / 4) of the quad, its element e = d % (D / 4), k-step e / 4; the four
@@ -613,53 +611,56 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(const KvAttnArgs a) {
   const int kvh = meta.y, n = meta.w;
   const int b = a.one ? (int)slot : kv_slot_seq_warp(a.s, slot, a.per, TILE, 1);
   KvSlot sl;
-  const int row0 = blockIdx.y * ROWS;
-  if (!kv_slot(a, slot, b, TILE, sl) || row0 >= sl.rows) return;
+  if (!kv_slot(a, slot, b, TILE, sl)) return;
   // the first part is in the slot that its worker says, the others are their worker's first segment
   auto part_of = [&](int i) { return a.part + (int64_t)(i == 0 ? meta.z : 2 * ((int)blockIdx.x + i)) * TILE * (D + 2); };
-  for (int r = warp; r < ROWS; r += 8) {
-    float m = -INFINITY, l = 0.f;
-    if (row0 + r < sl.rows) {
-      for (int i = lane; i < n; i += 32) {
-        const float x = part_of(i)[(int64_t)TILE * D + 2 * (row0 + r)];
-        factor[r][i] = x;
-        m = fmaxf(m, x);
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      for (int i = lane; i < n; i += 32) {
-        const float f = factor[r][i] == -INFINITY ? 0.f : kv_ex2(factor[r][i] - m);
-        factor[r][i] = f;
-        l = __fmaf_rn(f, part_of(i)[(int64_t)TILE * D + 2 * (row0 + r) + 1], l);
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    }
-    if (lane == 0) ml[r] = make_float2(m, l);
-  }
-  __syncthreads();
   // neighbours in a warp are rows where the parts are [chunk][row] (tiles of 256), chunks where they are [row][chunk]
-  const int r = TILE == 256 ? threadIdx.x % ROWS : threadIdx.x / CH, ch = TILE == 256 ? threadIdx.x / ROWS : threadIdx.x % CH;
-  if (row0 + r >= sl.rows) return;
-  const int64_t at = TILE == 256 ? ((int64_t)ch * TILE + row0 + r) * 4 : (int64_t)(row0 + r) * D + ch * 4;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const float f = factor[r][i];
-    const float4 v = *reinterpret_cast<const float4*>(part_of(i) + at);
-    if (f > 0.f) {  // a part that saw no key of the row may hold anything
-      o.x = __fmaf_rn(v.x, f, o.x);
-      o.y = __fmaf_rn(v.y, f, o.y);
-      o.z = __fmaf_rn(v.z, f, o.z);
-      o.w = __fmaf_rn(v.w, f, o.w);
+  const int tr = TILE == 256 ? threadIdx.x % ROWS : threadIdx.x / CH, ch = TILE == 256 ? threadIdx.x / ROWS : threadIdx.x % CH;
+  for (int row0 = blockIdx.y * ROWS; row0 < sl.rows; row0 += gridDim.y * ROWS) {
+    for (int r = warp; r < ROWS; r += 8) {
+      float m = -INFINITY, l = 0.f;
+      if (row0 + r < sl.rows) {
+        for (int i = lane; i < n; i += 32) {
+          const float x = part_of(i)[(int64_t)TILE * D + 2 * (row0 + r)];
+          factor[r][i] = x;
+          m = fmaxf(m, x);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int i = lane; i < n; i += 32) {
+          const float f = factor[r][i] == -INFINITY ? 0.f : kv_ex2(factor[r][i] - m);
+          factor[r][i] = f;
+          l = __fmaf_rn(f, part_of(i)[(int64_t)TILE * D + 2 * (row0 + r) + 1], l);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      }
+      if (lane == 0) ml[r] = make_float2(m, l);
     }
+    __syncthreads();
+    if (row0 + tr < sl.rows) {
+      const int64_t at = TILE == 256 ? ((int64_t)ch * TILE + row0 + tr) * 4 : (int64_t)(row0 + tr) * D + ch * 4;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float f = factor[tr][i];
+        const float4 v = *reinterpret_cast<const float4*>(part_of(i) + at);
+        if (f != 0.f) {  // a part that saw no key of the row may hold anything
+          o.x = __fmaf_rn(v.x, f, o.x);
+          o.y = __fmaf_rn(v.y, f, o.y);
+          o.z = __fmaf_rn(v.z, f, o.z);
+          o.w = __fmaf_rn(v.w, f, o.w);
+        }
+      }
+      kv_put_row(a, kv_row_out(a, sl, kvh, row0 + tr), ch, D, o, ml[tr].x, ml[tr].y);
+    }
+    __syncthreads();  // the factors are read
   }
-  kv_put_row(a, kv_row_out(a, sl, kvh, row0 + r), ch, D, o, ml[r].x, ml[r].y);
 }
 
 cudaError_t launch_kv_attn_join(const KvAttnArgs& a, int tile, cudaStream_t st) {
   if (a.workers > kMaxWorkers) return cudaErrorInvalidValue;
-  const dim3 grid((unsigned)(a.workers + (a.slots + 255) / 256), (unsigned)(tile / (1024 / a.c.dim)));
+  const dim3 grid((unsigned)(a.workers + (a.slots + 255) / 256), (unsigned)(tile == 256 ? 8 : tile / (1024 / a.c.dim) > 1 ? tile / (1024 / a.c.dim) : 1));
 #define H3Q_KV_J(DD, TT)                                     \
   if (a.c.dim == DD && tile == TT) {                         \
     kv_attn_join_kernel<DD, TT><<<grid, 256, 0, st>>>(a);    \
