@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(const KvAttnArgs a) {
 
 cudaError_t launch_kv_attn_join(const KvAttnArgs& a, int tile, cudaStream_t st) {
   if (a.workers > kMaxWorkers) return cudaErrorInvalidValue;
-  const dim3 grid((unsigned)(a.workers + (a.slots + 255) / 256), (unsigned)(tile == 256 ? 8 : tile / (1024 / a.c.dim) > 1 ? tile / (1024 / a.c.dim) : 1));
+  const dim3 grid((unsigned)(a.workers + (a.slots + 255) / 256), (unsigned)(tile == 256 ? 16 : tile / (1024 / a.c.dim) > 1 ? tile / (1024 / a.c.dim) : 1));
 #define H3Q_KV_J(DD, TT)                                     \
   if (a.c.dim == DD && tile == TT) {                         \
     kv_attn_join_kernel<DD, TT><<<grid, 256, 0, st>>>(a);    \

@@ -341,10 +341,10 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// heads a CTA takes: all of them where the pages alone fill the GPU (eight CTAs a multiprocessor), fewer where they do not
-int heads_each(const KvCache& c, int64_t slots) {
+// heads a CTA takes: all of them where the pages alone fill the GPU (2048 threads a multiprocessor), fewer where they do not
+int heads_each(const KvCache& c, int64_t slots, int threads) {
   int groups = 1;
-  while (groups < c.kv_heads && slots * 2 * groups < (int64_t)sm_count(0) * 8) ++groups;
+  while (groups < c.kv_heads && slots * 2 * groups * threads < (int64_t)sm_count(0) * 2048) ++groups;
   return (c.kv_heads + groups - 1) / groups;
 }
 
@@ -358,7 +358,7 @@ cudaError_t write_variant(const KvCache& c, const KvSeqs& s, const int32_t* past
     kv_write_few_kernel<KIND, CODES><<<(unsigned)((warps + 3) / 4), 128, 0, st>>>(c, s, past, k, v, vec, (uint32_t)slots);
     return cudaGetLastError();
   }
-  const int each = heads_each(c, slots);
+  const int each = heads_each(c, slots, c.page * c.dim <= 4096 ? 128 : c.page * c.dim / 32);
   const dim3 grid((unsigned)slots, (unsigned)((c.kv_heads + each - 1) / each), 2);
   switch (c.page * c.dim) {
     case 1024: kv_write_kernel<KIND, CODES, 128, 1><<<grid, 128, 0, st>>>(c, s, past, k, v, vec, each); break;
@@ -387,7 +387,7 @@ cudaError_t launch_kv_write(const KvCache& c, const KvSeqs& s, const int32_t* pa
 cudaError_t launch_kv_read(const KvCache& c, const KvSeqs& s, const int32_t* first, void* k_out, void* v_out, int kind,
                            cudaStream_t st) {
   const int64_t slots = (int64_t)s.tokens / c.page + 2 * (int64_t)s.batch;
-  const int each = heads_each(c, slots);
+  const int each = heads_each(c, slots, 256);
   const dim3 grid((unsigned)slots, (unsigned)((c.kv_heads + each - 1) / each), 2);
 #define H3Q_KV_R(K, C)                                                                 \
   if (kind == K && c.codes == C) {                                                     \

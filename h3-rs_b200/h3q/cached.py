@@ -1,0 +1,63 @@
+"""h3q.cached -- one attention layer of a text model that runs token by token or chunk by chunk: the library's linears and
+q / k RMSNorm + RoPE around the 8-bit key / value cache (h3q.kvcache).  The reference's text encoder sees its whole prompt at
+once (text.rs:377-395); this is the same layer with what came before kept in pages.
+
+    qkv = gemm_s8(x, qkv, rotate)                       [T, (heads + 2 kv_heads) * 128]
+    q, k = qk_norm_rope(qkv columns, rope rows of the tokens' positions)
+    write(cache, k, v)                                  behind the sequences' past tokens
+    att = attention(q, cache)                           each new token against all before it and itself
+    y = gemm_s8(att, out, rotate)
+
+A prompt goes in with its tokens at once, or a chunk a call; a generated token with one row a sequence; drafted tokens with
+a few.  Nothing here reads device memory on the host, so a step can be captured in a graph and replayed as past grows.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import gemm_s8, kvcache, qk_norm_rope
+from .dit import Linear
+
+
+@dataclass
+class Layer:
+    """qkv [(heads + 2 kv_heads) * 128, C] and out [C, heads * 128] are int8 ConvRot layers; q_norm, k_norm bf16 [128]."""
+    qkv: Linear
+    out: Linear
+    q_norm: object
+    k_norm: object
+    heads: int
+    kv_heads: int
+    rot: int = 128
+    eps: float = 1e-6
+
+
+def positions(past, tokens: int, starts=None):
+    """The position of each packed token: past[b] + its place among its sequence's new ones."""
+    at = torch.arange(tokens, device=past.device, dtype=torch.int32)
+    if starts is None:
+        each = tokens // past.numel()
+        return past.repeat_interleave(each, output_size=tokens) + at % each
+    seq = torch.searchsorted(starts[1:], at, right=True)
+    return past[seq] + at - starts[seq]
+
+
+def attend(x, layer: Layer, cache: kvcache.KVCache, page_table, past, rope, starts=None, max_new: int = 0):
+    """The layer on x bf16 [T, C], the new tokens of the sequences behind their past [batch] (int32) cached ones; rope f32
+    [2, positions, rot / 2].  Writes the tokens' keys and values into the cache; returns bf16 [T, C].  The caller moves
+    past on after the last layer."""
+    t, d, h, hk = x.shape[0], 128, layer.heads, layer.kv_heads
+    qkv = gemm_s8(x, layer.qkv.w, layer.qkv.ws, layer.qkv.bias, rotate=True)
+    cs = rope[:, positions(past, t, starts).long()].contiguous()
+    q = qk_norm_rope(qkv, 0, h, d, (layer.q_norm, layer.eps), cs, layer.rot)
+    k = qk_norm_rope(qkv, h * d, hk, d, (layer.k_norm, layer.eps), cs, layer.rot)
+    v = qkv[:, (h + hk) * d:].unflatten(1, (hk, d))
+    kvcache.write(cache, k, v, page_table, past, starts)
+    new = t // past.numel() if starts is None else starts[1:] - starts[:-1]
+    att = kvcache.attention(q, cache, page_table, past + new, starts, max_new=max_new)
+    return gemm_s8(att.reshape(t, h * d), layer.out.w, layer.out.ws, layer.out.bias, rotate=True)
+
+
+__all__ = ["Layer", "positions", "attend"]
