@@ -62,6 +62,8 @@ __device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
   return d;
 }
 
+// the n lowest bits (none for n <= 0, all from 32 on)
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }
 __device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(p)), "r"(bytes) : "memory");
 }
@@ -666,8 +668,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_wait_ld();
         if (edge) {
 #pragma unroll
-          for (int i = 0; i < BN; ++i)
-            if (i < a0 || i >= a1) x[i >> 5][i & 31] = 0xff800000u;
+          for (int k = 0; k < BN / 32; ++k) {  // a bit a score: predicates come from the bits several at a time
+            const uint32_t bits = below(a1 - 32 * k) & ~below(a0 - 32 * k);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[k][i] = bits >> i & 1 ? x[k][i] : 0xff800000u;
+          }
         }
         float mx = -INFINITY;
 #pragma unroll
