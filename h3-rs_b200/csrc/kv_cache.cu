@@ -69,6 +69,23 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a <= 3.402823466e38f ? a : 0.f;  // NaN and infinity compare false
 }
 
+// Magnitudes as bits, which order as the numbers do: NaN above infinity above the finite ones.  16-bit kinds keep two
+// running maxima in the halves of a word.
+template <int KIND>
+__device__ __forceinline__ void max_bits8(const Raw8<KIND>& r, uint32_t& m) {
+#pragma unroll
+  for (int i = 0; i < (KIND == 0 ? 8 : 4); ++i)
+    m = KIND == 0 ? max(m, r.w[i] & 0x7fffffffu) : __vmaxu2(m, r.w[i] & 0x7fff7fffu);
+}
+template <int KIND>
+__device__ __forceinline__ uint32_t whole_bits(uint32_t m) {  // the larger half, or the word
+  return KIND == 0 ? m : max(m & 0xffffu, m >> 16);
+}
+template <int KIND>
+__device__ __forceinline__ float bits_value(uint32_t m) {
+  return KIND == 0 ? __uint_as_float(m) : KIND == 1 ? h2f((uint16_t)m) : __uint_as_float(m << 16);
+}
+
 // the largest finite magnitude
 template <int KIND>
 __device__ __forceinline__ float amax8(const Raw8<KIND>& r) {
@@ -141,6 +158,35 @@ __device__ __forceinline__ uint2 requant8(uint2 w, float ratio) {
                                    __fmul_rn(g[3], ratio)));
 }
 
+// Codes of rows without NaN or infinity whose scale is at least their largest magnitude / top: no product is beyond
+// +-top by more than its rounding, so nothing saturates and int8 rounds by adding 1.5 * 2^23 (nearest even, as the
+// conversion does), which leaves the code in the low byte.
+template <int KIND, int CODES>
+__device__ __forceinline__ uint2 encode8_finite(const Raw8<KIND>& r, float inv) {
+  float f[8];
+  as_float8<KIND>(r, f);
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (CODES == kKvInt8) {
+      uint32_t q[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[e] = __float_as_uint(__fadd_rn(__fmul_rn(f[4 * i + e], inv), 12582912.f));
+      w[i] = prmt(prmt(q[0], q[1], 0x0040), prmt(q[2], q[3], 0x0040), 0x5410);
+    } else {
+      uint16_t lo, hi;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
+          : "=h"(lo)
+          : "f"(__fmul_rn(f[4 * i + 1], inv)), "f"(__fmul_rn(f[4 * i], inv)));
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
+          : "=h"(hi)
+          : "f"(__fmul_rn(f[4 * i + 3], inv)), "f"(__fmul_rn(f[4 * i + 2], inv)));
+      w[i] = (uint32_t)lo | ((uint32_t)hi << 16);
+    }
+  }
+  return make_uint2(w[0], w[1]);
+}
+
 template <int KIND, int CODES>
 __device__ __forceinline__ uint2 encode8(const Raw8<KIND>& r, float inv) {
   float f[8];
@@ -184,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, KIND == 0 ? 768 / THREADS : 1024 / TH
   if (w.page < 0) return;
   float* scale = (blockIdx.z ? c.v_scale : c.k_scale) + w.page * c.kv_heads;
   uint2* codes = reinterpret_cast<uint2*>((blockIdx.z ? c.v : c.k) + w.page * c.kv_heads * c.page * c.dim);
-  __shared__ float part[2][THREADS / 32];
+  __shared__ uint32_t part[2][THREADS / 32], again[THREADS / 32];
   float old = held ? scale[h0] : 0.f;
   for (int h = h0; h < h1; ++h) {
     const bool more = h + 1 < h1;
@@ -193,22 +239,35 @@ __global__ void __launch_bounds__(THREADS, KIND == 0 ? 768 / THREADS : 1024 / TH
       load(h + 1, y);
       old_next = held ? scale[h + 1] : 0.f;
     }
-    float m = 0.f;
+    uint32_t mb = 0;
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) m = fmaxf(m, amax8<KIND>(x[j]));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) part[h & 1][threadIdx.x >> 5] = m;
+    for (int j = 0; j < VPT; ++j) max_bits8<KIND>(x[j], mb);
+    mb = __reduce_max_sync(0xffffffffu, whole_bits<KIND>(mb));
+    if ((threadIdx.x & 31) == 0) part[h & 1][threadIdx.x >> 5] = mb;
     __syncthreads();  // one a head: the other half of `part` is not written before every thread has passed the next one
 #pragma unroll
-    for (int i = 0; i < THREADS / 32; ++i) m = fmaxf(m, part[h & 1][i]);
+    for (int i = 0; i < THREADS / 32; ++i) mb = max(mb, part[h & 1][i]);
+    float m = bits_value<KIND>(mb);
+    const bool finite = m <= 3.402823466e38f;
+    if (!finite) {  // rare: the maximum again, without what is not finite
+      m = 0.f;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) m = fmaxf(m, amax8<KIND>(x[j]));
+      mb = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+      if ((threadIdx.x & 31) == 0) again[threadIdx.x >> 5] = mb;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < THREADS / 32; ++i) mb = max(mb, again[i]);
+      m = __uint_as_float(mb);
+      __syncthreads();  // read before another head may come here
+    }
     const float now = fmaxf(old, fmaxf(__fmul_rn(m, 1.f / top_of(CODES)), kKvScaleFloor));
     const float inv = __fdiv_rn(1.f, now);
     uint2* dst = codes + (int64_t)h * (THREADS * VPT);
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int i = threadIdx.x + j * THREADS;
-      if (is_new(j)) dst[i] = encode8<KIND, CODES>(x[j], inv);
+      if (is_new(j)) dst[i] = finite ? encode8_finite<KIND, CODES>(x[j], inv) : encode8<KIND, CODES>(x[j], inv);
       else if (row0 + j * row_step < w.lo && now > old) dst[i] = requant8<CODES>(dst[i], __fdiv_rn(old, now));
     }
     if (threadIdx.x == 0) scale[h] = now;  // every thread has read the old scale of head h a head ago
