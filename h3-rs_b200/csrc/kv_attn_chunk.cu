@@ -9,12 +9,13 @@
 //                over the scores it came from (the A operand of the second product is read from there: with W in
 //                shared memory the products alone would take the SM's whole shared-memory bandwidth), row sums; the
 //                maximum moves only when a tile raises it by more than 2^8;
-//   warp 1       walks the work ahead of them: which rows and keys come next, and from the page table the address and
-//                the scales of each 16 keys, into rings in shared memory, so that the others never wait for a length
-//                or a table entry before they can ask for what it names;
-//   warps 12-15  widen codes to f16 into a ring of five 128-key tiles, K and V in turn: codes come straight from global memory into registers one tile ahead, K rows go out as
-//                they are, V is transposed on the way (byte permutes between eight keys of a thread), both in the
-//                K-major 128-byte-swizzle layout.
+//   warp 1       walks the work ahead of them: which rows and keys come next and, from the page table, the scales of each
+//                16 keys go into rings in shared memory, and the codes of two tiles ahead are copied there (cp.async.bulk),
+//                so that the others never wait for a length, a table entry or memory;
+//   warps 12-15  widen the codes to f16 into a ring of three 128-key tiles, K and V in turn: K rows go out as they are,
+//                V is transposed on the way (byte permutes between eight keys of a thread), both in the K-major
+//                128-byte-swizzle layout.  V's codes lie in groups of eight keys 16 bytes further apart than they are long,
+//                so that a warp reads eight groups at once without a bank conflict.
 // A page's scales never touch the codes (kv_attn.cuh).  Work is cut in 128-key tiles: a first kernel lists the slots
 // that have keys with their running sum, and the CTAs take equal contiguous ranges of the tiles of all (slot, kv head)
 // in order, so no wave is left part full; an item cut between CTAs is joined from f32 parts in order.
@@ -30,10 +31,10 @@ namespace {
 
 constexpr int BM = 128, BN = 128, NQ = 2, ROWS = NQ * BM;
 constexpr int THREADS = 512;
-constexpr int RING = 5, WR = 8;
-// setmaxnreg split of the 128 registers a thread at launch (512 x 128 = the whole file): MMA 48, softmax 2 x 184,
-// decode 96: 48 + 2 * 184 + 96 = 512 = 4 * 128.
-constexpr int REGS_MMA = 48, REGS_SOFT = 184, REGS_DEC = 96;
+constexpr int RING = 3, RAW = 2, WR = 8;
+// setmaxnreg split of the 128 registers a thread at launch (512 x 128 = the whole file): MMA and walker 48, softmax
+// 2 x 192, decode 80: 48 + 2 * 192 + 80 = 512 = 4 * 128.
+constexpr int REGS_MMA = 48, REGS_SOFT = 192, REGS_DEC = 80;
 static_assert(REGS_MMA + 2 * REGS_SOFT + REGS_DEC <= 4 * 128, "setmaxnreg split exceeds the launch");
 constexpr uint32_t TMEM_COLS = 512;
 constexpr float kMove = 8.f;
@@ -45,11 +46,15 @@ struct Cfg {
   static constexpr int KV_TILE = BN * D * 2;         // K: D / 64 slabs of 128 keys; V^T: 2 slabs of 64 keys x D
   static constexpr int V_SLAB = D * 128;
   static constexpr int OFF_KV = NQ * Q_TILE;
-  static constexpr int OFF_SC = OFF_KV + RING * KV_TILE;
-  static constexpr int OFF_ADDR = OFF_SC + WR * 8 * 16;
-  static constexpr int OFF_SEG = OFF_ADDR + WR * 8 * 8;
+  static constexpr int RAW_K = BN * D;               // codes of a tile
+  static constexpr int V_OCTET = 8 * D + 16;
+  static constexpr int RAW_V = 16 * V_OCTET;
+  static constexpr int OFF_RK = OFF_KV + RING * KV_TILE;
+  static constexpr int OFF_RV = OFF_RK + RAW * RAW_K;
+  static constexpr int OFF_SC = OFF_RV + RAW * RAW_V;
+  static constexpr int OFF_SEG = OFF_SC + WR * 8 * 16;
   static constexpr int OFF_BAR = OFF_SEG + 2 * 48;
-  static constexpr int NBAR = 2 * RING + 2 * WR + 4 * NQ + 1 + 4;
+  static constexpr int NBAR = 2 * RING + 4 * RAW + 2 * WR + 4 * NQ + 1 + 4;
   static constexpr size_t SMEM = 1024 + OFF_BAR + NBAR * 8 + 16;
   static_assert(SMEM + 16 <= 232448, "shared memory exceeds the sm_100 per-CTA limit");
 };
@@ -64,9 +69,6 @@ __device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
 
 // the n lowest bits (none for n <= 0, all from 32 on)
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1; }
-__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(p)), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 r;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
@@ -206,10 +208,13 @@ __global__ void __launch_bounds__(THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   float4* consts = reinterpret_cast<float4*>(smem + C::OFF_SC);  // [WR][8]: k scale, log2 of the v scale, its inverse
-  int64_t* addr = reinterpret_cast<int64_t*>(smem + C::OFF_ADDR);  // [WR][8]: offset of the codes of 16 keys, or -1
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* kv_empty = kv_full + RING;
-  uint64_t* wr_full = kv_empty + RING;
+  uint64_t* rk_full = kv_empty + RING;
+  uint64_t* rk_free = rk_full + RAW;
+  uint64_t* rv_full = rk_free + RAW;
+  uint64_t* rv_free = rv_full + RAW;
+  uint64_t* wr_full = rv_free + RAW;
   uint64_t* wr_free = wr_full + WR;
   uint64_t* q_full = wr_free + WR;
   uint64_t* s_full = q_full + NQ;
@@ -230,6 +235,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < RING; ++i) { mbar_init(&kv_full[i], 4); mbar_init(&kv_empty[i], 1); }
+    for (int i = 0; i < RAW; ++i) {
+      mbar_init(&rk_full[i], 1);
+      mbar_init(&rk_free[i], 4);
+      mbar_init(&rv_full[i], 1);
+      mbar_init(&rv_free[i], 4);
+    }
     for (int i = 0; i < WR; ++i) { mbar_init(&wr_full[i], 1); mbar_init(&wr_free[i], 4); }
     for (int t = 0; t < NQ; ++t) {
       mbar_init(&q_full[t], 4);
@@ -365,9 +376,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (wk.list[mid].before <= walk.x) walk.i = mid;
         else hi = mid;
       }
-      uint32_t tile = 0, si = 0;
+      uint32_t tile = 0, si = 0, asked_k = 0, asked_v = 0;
       bool ok = true;
-      Segment s;
+      Segment s{};
       auto hand = [&](int n) {  // stretch si to the others
         if (si >= 2 && !__all_sync(0xffffffffu, mbar_wait_prompt(&sg_free[si & 1], ((si >> 1) - 1) & 1, abort_flag, err,
                                                                  kDevTimeoutEmpty)))
@@ -398,36 +409,72 @@ __global__ void __launch_bounds__(THREADS, 1)
           cut = true;
         }
         if (!(ok = hand(s.t1 - s.t0))) break;
-        int64_t key = s.sl.lo + (int64_t)s.t0 * BN + lane * 16;
+        int64_t key = s.sl.lo + (int64_t)s.t0 * BN + (lane & 7) * 16;  // lane l + 8 does as lane l does
+        auto page_at = [&](int64_t k) { return k < s.sl.hi ? kv_page(a.c, a.s, s.sl.b, k >> a.c.page_log2) : (int64_t)-1; };
+        int64_t page_next = page_at(key);
         for (int j = s.t0; j < s.t1; ++j, ++tile, key += BN) {
-          const int64_t page = lane < 8 && key < s.sl.hi ? kv_page(a.c, a.s, s.sl.b, key >> a.c.page_log2) : -1;
-          int64_t off = -1;
+          const int64_t page = page_next, ph = page * a.c.kv_heads + s.kvh;
           float4 c = make_float4(0.f, -INFINITY, 0.f, 0.f);
           if (page >= 0) {
-            const int64_t ph = page * a.c.kv_heads + s.kvh;
-            off = (ph * a.c.page + (key & (a.c.page - 1))) * D;
-            // the decode warps ask for these codes three tiles from now, and find them in L2
-            prefetch_l2(a.c.k + off, 16 * D);
-            prefetch_l2(a.c.v + off, 16 * D);
             const float vs = fmaxf(__ldg(a.c.v_scale + ph), kKvScaleFloor);
             c = make_float4(__ldg(a.c.k_scale + ph), kv_lg2(vs), __fdividef(1.f, vs), 0.f);
           }
-          // entry tile - 8 is read once the decode warps may fill K of tile - 4: its ring slot held V of tile - 7, whose
-          // product is done
-          const uint32_t f = tile - 4;  // (a barrier a ring entry: the decode warps may be several tiles past f)
-          if (tile >= 4 && !__all_sync(0xffffffffu, mbar_wait_prompt(&wr_free[f % WR], (f / WR) & 1, abort_flag, err,
-                                                                      kDevTimeoutEmpty))) {
+          if (j + 1 < s.t1) page_next = page_at(key + BN);
+          const int64_t off = (ph * a.c.page + (key & (a.c.page - 1))) * D;  // of the lane's 16 keys' codes
+          // entry tile - 8 is read once the decode warps may fill K of tile - 4: its ring slot held V of tile - 6, whose
+          // product is done (a barrier a ring entry: the decode warps may be several tiles past f)
+          const uint32_t f = tile - 4;
+          const int r = tile % RAW;
+          const uint32_t freed = ((tile / RAW) & 1) ^ 1;
+          if ((tile >= 4 && !__all_sync(0xffffffffu, mbar_wait_prompt(&wr_free[f % WR], (f / WR) & 1, abort_flag, err,
+                                                                      kDevTimeoutEmpty))) ||
+              !__all_sync(0xffffffffu, mbar_wait_prompt(&rk_free[r], freed, abort_flag, err, kDevTimeoutEmpty))) {
             ok = false;
             break;
           }
-          if (lane < 8) {
-            consts[(tile % WR) * 8 + lane] = c;
-            addr[(tile % WR) * 8 + lane] = off;
+          if (lane < 8) consts[(tile % WR) * 8 + lane] = c;
+          // codes of 16 keys that are not there are zeros (their weights are, and 0 times what lay there may not be)
+          uint8_t* const rk = smem + C::OFF_RK + r * C::RAW_K;
+          uint8_t* const rv = smem + C::OFF_RV + r * C::RAW_V;
+          const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) & 0xffu;
+          auto zero = [&](uint8_t* at, int bytes) {
+            for (int i = lane * 16; i < bytes; i += 512) sts128(smem_u32(at + i), 0, 0, 0, 0);
+          };
+          for (uint32_t gone = ~there & 0xffu; gone; gone &= gone - 1) zero(rk + (__ffs(gone) - 1) * 16 * D, 16 * D);
+          fence_proxy_async_smem();  // zeros of an earlier tile come before the copies over them
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&wr_full[tile % WR]);
+            mbar_arrive_expect_tx(&rk_full[r], __popc(there) * 16 * D);
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&wr_full[tile % WR]);
+          if (lane < 8 && page >= 0) bulk_load_1d(rk + lane * 16 * D, a.c.k + off, 16 * D, &rk_full[r]);
+          ++asked_k;
+          if (!__all_sync(0xffffffffu, mbar_wait_prompt(&rv_free[r], freed, abort_flag, err, kDevTimeoutEmpty))) {
+            ok = false;
+            break;
+          }
+          for (uint32_t gone = ~there & 0xffu; gone; gone &= gone - 1) {
+            zero(rv + (__ffs(gone) - 1) * 2 * C::V_OCTET, 8 * D);
+            zero(rv + (__ffs(gone) - 1) * 2 * C::V_OCTET + C::V_OCTET, 8 * D);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(&rv_full[r], __popc(there) * 16 * D);
+          __syncwarp();
+          if (lane < 16 && page >= 0)  // lanes l and l + 8: the two octets of 16 keys
+            bulk_load_1d(rv + ((lane & 7) * 2 + (lane >> 3)) * C::V_OCTET, a.c.v + off + (lane >> 3) * 8 * D, 8 * D, &rv_full[r]);
+          ++asked_v;
         }
       }
+      // every copy asked for lands before the CTA ends
+      if (lane == 0) {
+        for (uint32_t t = asked_k < RAW ? 0 : asked_k - RAW; t < asked_k; ++t)
+          mbar_drain(&rk_full[t % RAW], (t / RAW) & 1, err, kDevTimeoutDrain);
+        for (uint32_t t = asked_v < RAW ? 0 : asked_v - RAW; t < asked_v; ++t)
+          mbar_drain(&rv_full[t % RAW], (t / RAW) & 1, err, kDevTimeoutDrain);
+      }
+      __syncwarp();
       if (lane == 0 && !cut) a.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
       if (ok) hand(0);
     }
@@ -442,104 +489,90 @@ __global__ void __launch_bounds__(THREADS, 1)
     // V: eight keys (octet vo of the tile) and D / 8 columns (chunk vc) a thread
     const int vo = (lane & 7) + 8 * (dw >> 1), vc = (lane >> 3) + 4 * (dw & 1);
     constexpr int VW = D / 32;                  // words of a chunk
-    uint4 kbuf[KP];
-    uint32_t vbuf[8][VW];
-    uint32_t seq = 0, tile0 = 0;
+    uint32_t seq = 0, tile = 0;
     bool ok = true;
     Stretch s;
-    for (uint32_t si = 0; ok && take_warp(si, s); ++si) {
-      const int n = s.n;
-      auto load_k = [&](int j) {
-        const uint32_t T = tile0 + j;
-        if (!__all_sync(0xffffffffu, mbar_wait_prompt(&wr_full[T % WR], (T / WR) & 1, abort_flag, err, kDevTimeoutScale)))
-          return false;
-#pragma unroll
-        for (int p = 0; p < KP; ++p) {
-          const int row = p * RPP + krow;
-          const int64_t off = addr[(T % WR) * 8 + (row >> 4)];
-          kbuf[p] = off < 0 ? make_uint4(0, 0, 0, 0)
-                            : __ldg(reinterpret_cast<const uint4*>(a.c.k + off + (row & 15) * D + kch * 16));
-        }
-        return true;
-      };
-      auto load_v = [&](int j) {
-        const int64_t off = addr[((tile0 + j) % WR) * 8 + (vo >> 1)];
-        const int64_t left = s.len - (s.key_base + (int64_t)j * BN + vo * 8);  // what lies behind the last token may be any bits
-        const uint8_t* src = a.c.v + (off < 0 ? 0 : off + (vo & 1) * 8 * D + vc * (D / 8));
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const bool there = off >= 0 && r < left;
-          if (VW == 4) {
-            const uint4 v = there ? __ldg(reinterpret_cast<const uint4*>(src + r * D)) : make_uint4(0, 0, 0, 0);
-            vbuf[r][0] = v.x;
-            vbuf[r][1] = v.y;
-            vbuf[r][VW - 2] = v.z;
-            vbuf[r][VW - 1] = v.w;
-          } else {
-            const uint2 v = there ? __ldg(reinterpret_cast<const uint2*>(src + r * D)) : make_uint2(0, 0);
-            vbuf[r][0] = v.x;
-            vbuf[r][1] = v.y;
-          }
-        }
-      };
-      auto wait_slot = [&]() {
-        return __all_sync(0xffffffffu, mbar_wait_prompt(&kv_empty[seq % RING], ((seq / RING) & 1) ^ 1, abort_flag, err,
-                                                         kDevTimeoutEmpty));
-      };
-      auto publish = [&]() {
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&kv_full[seq % RING]);
-        ++seq;
-      };
-      auto put_k = [&](int j) {
-        if (!wait_slot()) return false;
-        if (lane == 0) mbar_arrive(&wr_free[(tile0 + j) % WR]);
-        const uint32_t dst = smem_u32(smem + C::OFF_KV + (seq % RING) * C::KV_TILE);
-#pragma unroll
-        for (int p = 0; p < KP; ++p) {
-          uint32_t h[8];
-          kv_decode4<CODES>(kbuf[p].x, h[0], h[1]);
-          kv_decode4<CODES>(kbuf[p].y, h[2], h[3]);
-          kv_decode4<CODES>(kbuf[p].z, h[4], h[5]);
-          kv_decode4<CODES>(kbuf[p].w, h[6], h[7]);
-          const int row = p * RPP + krow, ch = (kch & 3) * 2;  // 16 columns: two 16-byte chunks of slab kch / 4
-          const uint32_t rb = dst + (kch >> 2) * C::Q_SLAB + row * 128;
-          sts128(rb + ((ch ^ (row & 7)) << 4), h[0], h[1], h[2], h[3]);
-          sts128(rb + (((ch + 1) ^ (row & 7)) << 4), h[4], h[5], h[6], h[7]);
-        }
-        publish();
-        return true;
-      };
-      auto put_v = [&]() {
-        if (!wait_slot()) return false;
-        const uint32_t dst = smem_u32(smem + C::OFF_KV + (seq % RING) * C::KV_TILE) + (vo >> 3) * C::V_SLAB;
-#pragma unroll
-        for (int q = 0; q < VW; ++q) {
-          uint32_t h[4][4];  // [column][key pair]
-#pragma unroll
-          for (int kp = 0; kp < 4; ++kp) {
-            kv_decode4<CODES>(prmt(vbuf[2 * kp][q], vbuf[2 * kp + 1][q], 0x5140), h[0][kp], h[1][kp]);
-            kv_decode4<CODES>(prmt(vbuf[2 * kp][q], vbuf[2 * kp + 1][q], 0x7362), h[2][kp], h[3][kp]);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int d = vc * (D / 8) + q * 4 + e;
-            sts128(dst + d * 128 + (((vo & 7) ^ (d & 7)) << 4), h[e][0], h[e][1], h[e][2], h[e][3]);
-          }
-        }
-        publish();
-        return true;
-      };
-      if (!(ok = load_k(0))) break;
-      load_v(0);
-      for (int j = 0; j < n; ++j) {
-        if (!(ok = put_k(j))) break;
-        if (j + 1 < n && !(ok = load_k(j + 1))) break;
-        if (!(ok = put_v())) break;
-        if (j + 1 < n) load_v(j + 1);
+    // a free place in the ring, and the codes that go there
+    auto wait_both = [&](uint64_t* full) {
+      return __all_sync(0xffffffffu,
+                        mbar_wait_prompt(&kv_empty[seq % RING], ((seq / RING) & 1) ^ 1, abort_flag, err, kDevTimeoutEmpty) &&
+                            mbar_wait_prompt(full, (tile / RAW) & 1, abort_flag, err, kDevTimeoutFull));
+    };
+    auto publish = [&](uint64_t* free) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(free);
+        mbar_arrive(&kv_full[seq % RING]);
       }
-      tile0 += n;
+      ++seq;
+    };
+    for (uint32_t si = 0; ok && take_warp(si, s); ++si) {
+      for (int j = 0; j < s.n; ++j, ++tile) {
+        const int r = tile % RAW;
+        if (!(ok = wait_both(&rk_full[r]))) break;
+        if (lane == 0) mbar_arrive(&wr_free[tile % WR]);
+        {
+          const uint32_t dst = smem_u32(smem + C::OFF_KV + (seq % RING) * C::KV_TILE);
+          const uint32_t src = smem_u32(smem + C::OFF_RK + r * C::RAW_K) + krow * D + kch * 16;
+          const bool odd = kch >= 4;  // the second slab's lanes store their pieces in the other order: no two meet in a bank
+#pragma unroll
+          for (int p = 0; p < KP; ++p) {
+            const uint4 v = lds128(src + p * RPP * D);
+            uint32_t h[8];
+            kv_decode4<CODES>(odd ? v.z : v.x, h[0], h[1]);
+            kv_decode4<CODES>(odd ? v.w : v.y, h[2], h[3]);
+            kv_decode4<CODES>(odd ? v.x : v.z, h[4], h[5]);
+            kv_decode4<CODES>(odd ? v.y : v.w, h[6], h[7]);
+            const int row = p * RPP + krow, ch = (kch & 3) * 2 + odd;  // 16 columns: two 16-byte chunks of slab kch / 4
+            const uint32_t rb = dst + (kch >> 2) * C::Q_SLAB + row * 128;
+            sts128(rb + ((ch ^ (row & 7)) << 4), h[0], h[1], h[2], h[3]);
+            sts128(rb + (((ch ^ 1) ^ (row & 7)) << 4), h[4], h[5], h[6], h[7]);
+          }
+        }
+        publish(&rk_free[r]);
+        if (!(ok = wait_both(&rv_full[r]))) break;
+        {
+          const uint32_t dst = smem_u32(smem + C::OFF_KV + (seq % RING) * C::KV_TILE) + (vo >> 3) * C::V_SLAB;
+          const uint32_t src = smem_u32(smem + C::OFF_RV + r * C::RAW_V) + vo * C::V_OCTET + vc * (D / 8);
+          uint32_t v[8][VW];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (VW == 4) {
+              const uint4 q = lds128(src + e * D);
+              v[e][0] = q.x;
+              v[e][1] = q.y;
+              v[e][VW - 2] = q.z;
+              v[e][VW - 1] = q.w;
+            } else {
+              asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[e][0]), "=r"(v[e][1]) : "r"(src + e * D) : "memory");
+            }
+          }
+          const int64_t left = s.len - (s.key_base + (int64_t)j * BN + vo * 8);
+          if (left < 8) {  // what lies behind the last token may be any bits
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (e >= left)
+#pragma unroll
+                for (int q = 0; q < VW; ++q) v[e][q] = 0;
+          }
+#pragma unroll
+          for (int q = 0; q < VW; ++q) {
+            uint32_t h[4][4];  // [column][key pair]
+#pragma unroll
+            for (int kp = 0; kp < 4; ++kp) {
+              kv_decode4<CODES>(prmt(v[2 * kp][q], v[2 * kp + 1][q], 0x5140), h[0][kp], h[1][kp]);
+              kv_decode4<CODES>(prmt(v[2 * kp][q], v[2 * kp + 1][q], 0x7362), h[2][kp], h[3][kp]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int d = vc * (D / 8) + q * 4 + e;
+              sts128(dst + d * 128 + (((vo & 7) ^ (d & 7)) << 4), h[e][0], h[e][1], h[e][2], h[e][3]);
+            }
+          }
+        }
+        publish(&rv_free[r]);
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFT));
