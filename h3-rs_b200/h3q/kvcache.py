@@ -59,8 +59,16 @@ class KVCache:
         return cls(codes[0], codes[1], scales[0], scales[1])
 
 
-def _stream(cache) -> int:
-    return torch._C._cuda_getCurrentRawStream(cache.device)
+def _call(cache, name, *args) -> None:
+    """One call of the library on the current stream of the cache's device."""
+    stream = torch._C._cuda_getCurrentRawStream(cache.device)
+    if torch._C._cuda_getDevice() == cache.device:
+        status = getattr(lib(), name)(cache.ref, *args, stream)
+    else:
+        with torch.cuda.device(cache.device):
+            status = getattr(lib(), name)(cache.ref, *args, stream)
+    if status:
+        check(status)
 
 
 def _ints(name, t, cache, n):
@@ -109,10 +117,7 @@ def write(cache: KVCache, k, v, page_table, past, starts=None) -> None:
     table, batch, width = _table(page_table, cache)
     pp = _ints("past", past, cache, batch)
     sp = _ints("starts", starts, cache, batch + 1)
-    st = lib().h3q_kv_write(cache.ref, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, kind, k.shape[0], table, width, pp, sp,
-                            batch, _stream(cache))
-    if st:
-        check(st)
+    _call(cache, "h3q_kv_write", k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, kind, k.shape[0], table, width, pp, sp, batch)
 
 
 def read(cache: KVCache, page_table, starts, total: int, dtype=torch.bfloat16, first=None):
@@ -125,9 +130,7 @@ def read(cache: KVCache, page_table, starts, total: int, dtype=torch.bfloat16, f
     shape = (total, cache.heads, cache.dim)
     k = cache.k.new_empty(shape, dtype=dtype)
     v = torch.empty_like(k)
-    st = lib().h3q_kv_read(cache.ref, table, width, fp, sp, batch, total, k.data_ptr(), v.data_ptr(), kind, _stream(cache))
-    if st:
-        check(st)
+    _call(cache, "h3q_kv_read", table, width, fp, sp, batch, total, k.data_ptr(), v.data_ptr(), kind)
     return k, v
 
 
@@ -149,15 +152,12 @@ def attention(q, cache: KVCache, page_table, lengths, starts=None, scale: float 
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     if starts is None and batch:
         max_new = tokens // batch
-    L = lib()
-    need = L.h3q_kv_attention_workspace_size(tokens, batch, heads, cache.heads, dim, max_new)
+    need = lib().h3q_kv_attention_workspace_size(tokens, batch, heads, cache.heads, dim, max_new)
     if workspace is None or workspace.numel() < need:
         workspace = q.new_empty(need, dtype=torch.uint8)
-    st = L.h3q_kv_attention(cache.ref, q.data_ptr(), _KIND[q.dtype], qt, qh, tokens, heads, table, width, lp, sp, batch,
-                            max_new, dim ** -0.5 if scale is None else scale, causal, window, out.data_ptr(),
-                            lse.data_ptr() if return_lse else None, workspace.data_ptr(), workspace.numel(), _stream(cache))
-    if st:
-        check(st)
+    _call(cache, "h3q_kv_attention", q.data_ptr(), _KIND[q.dtype], qt, qh, tokens, heads, table, width, lp, sp, batch, max_new,
+          dim ** -0.5 if scale is None else scale, causal, window, out.data_ptr(), lse.data_ptr() if return_lse else None,
+          workspace.data_ptr(), workspace.numel())
     return (out, lse) if return_lse else out
 
 

@@ -180,6 +180,18 @@ def test_attention(cuda, case):
                   max_new=max(news) if case % 2 else 0, strided=case % 3 == 1)
 
 
+@pytest.mark.parametrize("new", [1, 9, 200])
+def test_attention_of_rows_that_are_not_aligned(cuda, new):
+    """q begins 2 bytes behind a 16-byte boundary and its rows lie an odd number of elements apart."""
+    totals = [new + 77]
+    cache, table = make_cache(cuda, I8, 2, 32, 128, totals, 12)
+    flat = torch.randn(1 + new * (4 * 128 + 3), generator=_gen(1, cuda), device=cuda).to(BF)
+    q = flat[1:].view(new, 4 * 128 + 3)[:, :512].unflatten(1, (4, 128))
+    n = _i32(totals, cuda)
+    assert q.data_ptr() % 16 == 2 and (new == 1 or q.stride(0) == 515)
+    assert torch.equal(kvcache.attention(q, cache, table, n), kvcache.attention(q.contiguous(), cache, table, n))
+
+
 @pytest.mark.parametrize("new", [1, 3, 40])
 def test_attention_without_starts(cuda, new):
     run_attention(cuda, I8, BF, 2, 4, 128, 64, [100, 70, 333], [new] * 3, seed=new, starts=False)
@@ -405,6 +417,19 @@ def test_write_of_rows_that_are_not_finite(cuda, codes, n):
     assert abs(float(s) - float(clean.abs().max()) / TOP[codes]) <= 4 * 2.0 ** -24 * float(s)
     assert k[0, 0, 3] == 0 and k[0, 0, 5] == TOP[codes] * s and k[0, 0, 7] == -TOP[codes] * s
     assert (k[:, 1] == 0).all() and float(cache.k_scale[1, 1]) == pytest.approx(1e-30, rel=1e-6)
+
+
+def test_places_outside_the_table(cuda):
+    """Tokens before place 0 or behind the table's last page read as zeros and are dropped when written."""
+    cache, table = make_cache(cuda, I8, 1, 16, 64, [32], 3, spare=0)  # one page more in the table, which names none
+    starts = _i32([0, 60], cuda)
+    k, _ = kvcache.read(cache, table, starts, 60, torch.float32, _i32([-10], cuda))
+    all32, _ = kvcache.read(cache, table, _i32([0, 32], cuda), 32, torch.float32)
+    assert (k[:10] == 0).all() and torch.equal(k[10:42], all32) and (k[42:] == 0).all()
+    x = torch.ones((60, 1, 64), device=cuda)
+    kvcache.write(cache, x, x, table, _i32([-10], cuda), starts)
+    k, _ = kvcache.read(cache, table, _i32([0, 32], cuda), 32, torch.float32)
+    assert ((k - 1).abs() <= 2.0 ** -22).all()
 
 
 def test_read_spans(cuda):
