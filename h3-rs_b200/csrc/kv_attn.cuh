@@ -37,7 +37,8 @@ struct KvAttnArgs {
   int4* meta;              // [workers]: slot, kv head, first part and parts of the item that w began and did not finish
   int workers;
 };
-constexpr int kMaxWorkers = 256;  // one a multiprocessor
+constexpr int kMaxWorkers = 256;         // of the chunk kernel: one a multiprocessor
+constexpr int kMaxRowWorkers = 512;      // of the row kernel: up to three
 
 // What a slot stands for: `rows` query rows of sequence b, (token, head of the group) in that order, and the keys
 // [lo, hi) that any of them sees, lo a multiple of 16.

@@ -9,10 +9,20 @@
 // d = 16 g .. 16 g + 15 of keys 2t, 2t + 1, 2t + 8, 2t + 9.  The ring is swizzled so that both reads are free of
 // bank conflicts.
 //
-// Work is cut by keys, not by sequences: the units (128 keys of a sequence and kv head) of the whole call, in order,
-// are dealt to the CTAs in equal contiguous ranges.  A CTA's warps take the 16-key steps of a range in turn and
+// Work is cut by keys, not by sequences: the units (64 keys of a sequence and kv head) of the whole call, in order,
+// are dealt to the CTAs in equal contiguous ranges.  A CTA's four warps take the 16-key steps of a range in turn and
 // join their running (m, l, O) at its end; a (sequence, kv head) cut between CTAs goes through f32 parts in the
-// workspace, joined in order by a second kernel, so results do not depend on timing.
+// workspace, joined in order by a second kernel, so results do not depend on timing.  The chain of loads at the begin
+// of a range's next sequence (lengths, page table, codes) takes about 3 us; three CTAs a multiprocessor (two of 32 rows) hide it
+// behind each other's work, which one CTA of twelve warps could not, not even by starting it ahead of the join (64
+// sequences of 1024 tokens, 8 kv heads: 52.4 us with one CTA, 53.7 with the early start, 40.2 with three; two warps and
+// six CTAs: 39.4, but 5 us more to join and 47.9 against 40.8 us for 25 rows).
+//
+// Measured (B200; head dim 128, 8 kv heads): one token of 64 sequences of up to 16384, int8, 5 query heads to a kv head,
+// 1.2 GB: 224 us, 5.4 TB/s; one of a sequence of 131000, 268 MB: 57 us, 4.7 TB/s; five of 16 sequences of up to 4099
+// (25 rows), e4m3: 41 us.  The copies alone reach 6.1 TB/s in the first: what keeps the rest is the widening of codes (a third
+// of the ALU pipe, five instructions for four codes) and its latencies, with 12 warps a multiprocessor for their
+// registers.  Tried and slower: scores in two accumulator chains (spills), two steps at a time (spills), 14 warps.
 #include <cstdint>
 #include <cuda_runtime.h>
 #include "kv_attn.cuh"
@@ -26,7 +36,8 @@ constexpr float kMove = 8.f;        // log2 of the largest weight between moves 
 
 template <int D, int MT>
 struct RowsCfg {
-  static constexpr int kWarps = MT == 1 ? 12 : 8, kThreads = kWarps * 32;
+  static constexpr int kWarps = 4, kThreads = kWarps * 32;
+  static constexpr int kCtas = MT == 1 ? 3 : 2;    // of a multiprocessor
   static constexpr int kUnit = kWarps * 16;  // keys of a unit
   static constexpr int kStages = MT == 1 ? 3 : 4;
   static constexpr int kStageBytes = 2 * 16 * D;           // K and V codes of 16 keys
@@ -119,7 +130,7 @@ __device__ __forceinline__ int sched_load(const KvAttnArgs& a, Sched<W>& sc, int
 }
 
 template <int D, int CODES, int MT>
-__global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, 1) kv_attn_rows_kernel(const KvAttnArgs a) {
+__global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCtas) kv_attn_rows_kernel(const KvAttnArgs a) {
   using C = RowsCfg<D, MT>;
   constexpr int TILE = MT * 16, NT = D / 8, kWarps = C::kWarps, kThreads = C::kThreads, kUnit = C::kUnit;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -560,10 +571,11 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, 1) kv_attn_rows_kern
 // thread takes four columns of a row and adds the parts in their order, each with its factor 2^(m_i - m).  The blocks
 // after them look through the slots for those without any key, whose rows are zeros, and for sequences that no kernel of
 // the call takes, whose rows are NaN.
+// Latency: 4 to 5 us for most calls, 9 us for a sequence of 131000 in 55 parts a kv head (14.5 us with four loads in flight).
 template <int D, int TILE>
-__global__ void __launch_bounds__(256) kv_attn_join_kernel(const KvAttnArgs a) {
+__global__ void __launch_bounds__(256, 4) kv_attn_join_kernel(const KvAttnArgs a) {
   constexpr int CH = D / 4, ROWS = 256 / CH;  // 16-byte chunks of a row, rows of a block
-  __shared__ float factor[ROWS][kMaxWorkers];
+  __shared__ float factor[ROWS][TILE == 256 ? kMaxWorkers : kMaxRowWorkers];
   __shared__ float2 ml[ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if ((int)blockIdx.x >= a.workers) {
@@ -641,15 +653,21 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(const KvAttnArgs a) {
     if (row0 + tr < sl.rows) {
       const int64_t at = TILE == 256 ? ((int64_t)ch * TILE + row0 + tr) * 4 : (int64_t)(row0 + tr) * D + ch * 4;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float f = factor[tr][i];
-        const float4 v = *reinterpret_cast<const float4*>(part_of(i) + at);
-        if (f != 0.f) {  // a part that saw no key of the row may hold anything
-          o.x = __fmaf_rn(v.x, f, o.x);
-          o.y = __fmaf_rn(v.y, f, o.y);
-          o.z = __fmaf_rn(v.z, f, o.z);
-          o.w = __fmaf_rn(v.w, f, o.w);
+      constexpr int AT_ONCE = TILE == 256 ? 4 : 8;   // loads in flight: an item of few rows may have hundreds of parts
+      for (int i0 = 0; i0 < n; i0 += AT_ONCE) {
+        float4 v[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u)
+          if (i0 + u < n) v[u] = *reinterpret_cast<const float4*>(part_of(i0 + u) + at);
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+          const float f = i0 + u < n ? factor[tr][i0 + u] : 0.f;
+          if (f != 0.f) {  // a part that saw no key of the row may hold anything
+            o.x = __fmaf_rn(v[u].x, f, o.x);
+            o.y = __fmaf_rn(v[u].y, f, o.y);
+            o.z = __fmaf_rn(v[u].z, f, o.z);
+            o.w = __fmaf_rn(v[u].w, f, o.w);
+          }
         }
       }
       kv_put_row(a, kv_row_out(a, sl, kvh, row0 + tr), ch, D, o, ml[tr].x, ml[tr].y);
@@ -659,7 +677,7 @@ __global__ void __launch_bounds__(256) kv_attn_join_kernel(const KvAttnArgs a) {
 }
 
 cudaError_t launch_kv_attn_join(const KvAttnArgs& a, int tile, cudaStream_t st) {
-  if (a.workers > kMaxWorkers) return cudaErrorInvalidValue;
+  if (a.workers > (tile == 256 ? kMaxWorkers : kMaxRowWorkers)) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)(a.workers + (a.slots + 255) / 256), (unsigned)(tile == 256 ? 16 : tile / (1024 / a.c.dim) > 1 ? tile / (1024 / a.c.dim) : 1));
 #define H3Q_KV_J(DD, TT)                                     \
   if (a.c.dim == DD && tile == TT) {                         \
@@ -686,7 +704,7 @@ cudaError_t launch_rows(KvAttnArgs a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     ready[dev] = true;
   }
-  a.workers = sm_count(dev);
+  a.workers = sm_count(dev) * C::kCtas;
   kern<<<(unsigned)a.workers, C::kThreads, C::kSmem, st>>>(a);
   if (const cudaError_t e = cudaGetLastError()) return e;
   return launch_kv_attn_join(a, MT * 16, st);
@@ -694,7 +712,7 @@ cudaError_t launch_rows(KvAttnArgs a, cudaStream_t st) {
 
 }  // namespace
 
-size_t kv_attn_rows_part_bytes(int dim, int tile) { return (size_t)kMaxWorkers * 2 * tile * (dim + 2) * 4; }
+size_t kv_attn_rows_part_bytes(int dim, int tile) { return (size_t)kMaxRowWorkers * 2 * tile * (dim + 2) * 4; }
 
 // tile: 16 or 32 rows
 cudaError_t launch_kv_attn_rows(const KvAttnArgs& a, int tile, cudaStream_t st) {

@@ -125,7 +125,7 @@ AttnPlan plan(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_heads, in
   if (p.tile) {
     p.slots = batch;
     p.part = a256(kv_attn_rows_part_bytes(dim, p.tile));
-    p.meta = a256(kMaxWorkers * sizeof(int4));
+    p.meta = a256(kMaxRowWorkers * sizeof(int4));
   }
   if (p.chunk) {
     p.chunk_slots = tokens * per / 256 + batch;
