@@ -571,11 +571,15 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
 // thread takes four columns of a row and adds the parts in their order, each with its factor 2^(m_i - m).  The blocks
 // after them look through the slots for those without any key, whose rows are zeros, and for sequences that no kernel of
 // the call takes, whose rows are NaN.
-// Latency: 4 to 5 us for most calls, 9 us for a sequence of 131000 in 55 parts a kv head (14.5 us with four loads in flight).
+// Latency: 4 to 5 us for most calls of few rows, 11 us for a sequence of 131000 in 55 parts a kv head (14.5 us with four
+// loads in flight); 15 us for the 148 items of 256 rows of head dim 128 that a large chunk call cuts (23 us with a block for eight
+// rows instead of 32).
 template <int D, int TILE>
 __global__ void __launch_bounds__(256, 4) kv_attn_join_kernel(const KvAttnArgs a) {
-  constexpr int CH = D / 4, ROWS = 256 / CH;  // 16-byte chunks of a row, rows of a block
-  __shared__ float factor[ROWS][TILE == 256 ? kMaxWorkers : kMaxRowWorkers];
+  // 16-byte chunks of a row; rows of a block, those of a thread BY apart; loads of a thread in flight: a large tile has many
+  // rows of few parts, a small one few rows of, at times, hundreds
+  constexpr int CH = D / 4, BY = 256 / CH, R = TILE == 256 ? 4 : 1, ROWS = BY * R, AT_ONCE = 8 / R;
+  constexpr int LANES = TILE == 256 ? 8 : 32;  // that look at the statistics of a row's parts
   __shared__ float2 ml[ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if ((int)blockIdx.x >= a.workers) {
@@ -626,59 +630,73 @@ __global__ void __launch_bounds__(256, 4) kv_attn_join_kernel(const KvAttnArgs a
   if (!kv_slot(a, slot, b, TILE, sl)) return;
   // the first part is in the slot that its worker says, the others are their worker's first segment
   auto part_of = [&](int i) { return a.part + (int64_t)(i == 0 ? meta.z : 2 * ((int)blockIdx.x + i)) * TILE * (D + 2); };
+  auto ml_of = [&](int i, int row) { return reinterpret_cast<const float2*>(part_of(i) + (int64_t)TILE * D) + row; };
   // neighbours in a warp are rows where the parts are [chunk][row] (tiles of 256), chunks where they are [row][chunk]
-  const int tr = TILE == 256 ? threadIdx.x % ROWS : threadIdx.x / CH, ch = TILE == 256 ? threadIdx.x / ROWS : threadIdx.x % CH;
+  const int tr = TILE == 256 ? threadIdx.x % BY : threadIdx.x / CH, ch = TILE == 256 ? threadIdx.x / BY : threadIdx.x % CH;
   for (int row0 = blockIdx.y * ROWS; row0 < sl.rows; row0 += gridDim.y * ROWS) {
-    for (int r = warp; r < ROWS; r += 8) {
+    for (int r = threadIdx.x / LANES; r < ROWS; r += 256 / LANES) {
       float m = -INFINITY, l = 0.f;
-      if (row0 + r < sl.rows) {
-        for (int i = lane; i < n; i += 32) {
-          const float x = part_of(i)[(int64_t)TILE * D + 2 * (row0 + r)];
-          factor[r][i] = x;
-          m = fmaxf(m, x);
+      if (row0 + r < sl.rows)
+        for (int i = lane % LANES; i < n; i += LANES) {
+          const float2 e = __ldg(ml_of(i, row0 + r));
+          const float to = fmaxf(m, e.x);
+          l *= m == -INFINITY ? 0.f : kv_ex2(m - to);
+          l = __fmaf_rn(e.x == -INFINITY ? 0.f : kv_ex2(e.x - to), e.y, l);
+          m = to;
         }
 #pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        for (int i = lane; i < n; i += 32) {
-          const float f = factor[r][i] == -INFINITY ? 0.f : kv_ex2(factor[r][i] - m);
-          factor[r][i] = f;
-          l = __fmaf_rn(f, part_of(i)[(int64_t)TILE * D + 2 * (row0 + r) + 1], l);
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      for (int o = LANES / 2; o; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o), to = fmaxf(m, m2);
+        const float f = m == -INFINITY ? 0.f : kv_ex2(m - to), f2 = m2 == -INFINITY ? 0.f : kv_ex2(m2 - to);
+        l = __fadd_rn(__fmul_rn(l, f), __fmul_rn(l2, f2));  // the same in both lanes
+        m = to;
       }
-      if (lane == 0) ml[r] = make_float2(m, l);
+      if (lane % LANES == 0) ml[r] = make_float2(m, l);
     }
     __syncthreads();
-    if (row0 + tr < sl.rows) {
-      const int64_t at = TILE == 256 ? ((int64_t)ch * TILE + row0 + tr) * 4 : (int64_t)(row0 + tr) * D + ch * 4;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      constexpr int AT_ONCE = TILE == 256 ? 4 : 8;   // loads in flight: an item of few rows may have hundreds of parts
-      for (int i0 = 0; i0 < n; i0 += AT_ONCE) {
-        float4 v[AT_ONCE];
+    float4 o[R];
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u)
-          if (i0 + u < n) v[u] = *reinterpret_cast<const float4*>(part_of(i0 + u) + at);
+    for (int k = 0; k < R; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = 0; i0 < n; i0 += AT_ONCE) {
+      float4 v[AT_ONCE][R];
+      float f[AT_ONCE][R];
 #pragma unroll
-        for (int u = 0; u < AT_ONCE; ++u) {
-          const float f = i0 + u < n ? factor[tr][i0 + u] : 0.f;
-          if (f != 0.f) {  // a part that saw no key of the row may hold anything
-            o.x = __fmaf_rn(v[u].x, f, o.x);
-            o.y = __fmaf_rn(v[u].y, f, o.y);
-            o.z = __fmaf_rn(v[u].z, f, o.z);
-            o.w = __fmaf_rn(v[u].w, f, o.w);
+      for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          const int row = row0 + tr + k * BY;
+          f[u][k] = -INFINITY;
+          if (i0 + u < n && row < sl.rows) {
+            const int64_t at = TILE == 256 ? ((int64_t)ch * TILE + row) * 4 : (int64_t)row * D + ch * 4;
+            v[u][k] = *reinterpret_cast<const float4*>(part_of(i0 + u) + at);
+            f[u][k] = __ldg(&ml_of(i0 + u, row)->x);
           }
         }
-      }
-      kv_put_row(a, kv_row_out(a, sl, kvh, row0 + tr), ch, D, o, ml[tr].x, ml[tr].y);
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          const float w = f[u][k] == -INFINITY ? 0.f : kv_ex2(f[u][k] - ml[tr + k * BY].x);
+          if (w != 0.f) {  // a part that saw no key of the row may hold anything
+            o[k].x = __fmaf_rn(v[u][k].x, w, o[k].x);
+            o[k].y = __fmaf_rn(v[u][k].y, w, o[k].y);
+            o[k].z = __fmaf_rn(v[u][k].z, w, o[k].z);
+            o[k].w = __fmaf_rn(v[u][k].w, w, o[k].w);
+          }
+        }
     }
-    __syncthreads();  // the factors are read
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const int row = row0 + tr + k * BY;
+      if (row < sl.rows) kv_put_row(a, kv_row_out(a, sl, kvh, row), ch, D, o[k], ml[tr + k * BY].x, ml[tr + k * BY].y);
+    }
+    __syncthreads();  // the statistics are read
   }
 }
 
 cudaError_t launch_kv_attn_join(const KvAttnArgs& a, int tile, cudaStream_t st) {
   if (a.workers > (tile == 256 ? kMaxWorkers : kMaxRowWorkers)) return cudaErrorInvalidValue;
-  const dim3 grid((unsigned)(a.workers + (a.slots + 255) / 256), (unsigned)(tile == 256 ? 16 : tile / (1024 / a.c.dim) > 1 ? tile / (1024 / a.c.dim) : 1));
+  const dim3 grid((unsigned)(a.workers + (a.slots + 255) / 256), (unsigned)(tile == 256 ? a.c.dim / 16 : tile / (1024 / a.c.dim) > 1 ? tile / (1024 / a.c.dim) : 1));
 #define H3Q_KV_J(DD, TT)                                     \
   if (a.c.dim == DD && tile == TT) {                         \
     kv_attn_join_kernel<DD, TT><<<grid, 256, 0, st>>>(a);    \
