@@ -20,7 +20,6 @@ from h3q import kvcache
 pytestmark = pytest.mark.gpu
 
 TOP = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
-STEP = {torch.int8: 1.0, torch.float8_e4m3fn: None}
 
 
 def _gen(seed, dev):
@@ -301,10 +300,6 @@ def test_attention_beyond_32_bit_offsets(cuda):
 
 
 # ---------------------------------------------------------------------------------------------------- write and read
-
-def e4m3(x):
-    return x.float().to(torch.float8_e4m3fn).double()
-
 
 def _steps(codes, code):
     """The spacing of the code type around `code` (at least that of its smallest numbers)."""
