@@ -14,7 +14,7 @@ the host never reads.  Calls run on the current stream of the cache's device.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
+import functools
 
 import torch
 
@@ -24,31 +24,30 @@ _KIND = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _CODES = {torch.int8: KV_INT8, torch.float8_e4m3fn: KV_E4M3}
 
 
-@dataclass
 class KVCache:
-    """k, v codes [pages, kv_heads, page, head_dim] (int8 or float8_e4m3fn), k_scale, v_scale f32 [pages, kv_heads]."""
-    k: torch.Tensor
-    v: torch.Tensor
-    k_scale: torch.Tensor
-    v_scale: torch.Tensor
+    """k, v codes [pages, kv_heads, page, head_dim] (int8 or float8_e4m3fn), k_scale, v_scale f32 [pages, kv_heads].  The
+    tensors are checked once, here, and stay: others need another KVCache."""
 
-    def __post_init__(self):
-        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
+    def __init__(self, k, v, k_scale, v_scale):
         shape, code = k.shape, _CODES.get(k.dtype)
         if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype:
             raise H3QError(ERR_ARG, "KVCache: k and v are codes [pages, kv_heads, page, head_dim] of one type")
         if code is None:
             raise H3QError(ERR_ARG, "KVCache: codes are int8 or float8_e4m3fn")
-        if ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.shape != shape[:2] or vs.shape != shape[:2]:
+        pages, heads, page, dim = shape
+        f32, scales = torch.float32, (pages, heads)
+        if k_scale.dtype != f32 or v_scale.dtype != f32 or k_scale.shape != scales or v_scale.shape != scales:
             raise H3QError(ERR_ARG, "KVCache: scales are f32 [pages, kv_heads]")
-        self.device = k.get_device()  # -1: not a CUDA tensor
-        if self.device < 0 or not (v.get_device() == ks.get_device() == vs.get_device() == self.device) or not (
-                k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        device = k.get_device()  # -1: not a CUDA tensor
+        if device < 0 or not (v.get_device() == k_scale.get_device() == v_scale.get_device() == device) or not (
+                k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
             raise ValueError("h3q: expected contiguous CUDA tensors of one device")
-        pages, self.heads, page, self.dim = shape
-        self.desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), pages, self.heads, page, self.dim,
-                                code)
-        self.ref = ctypes.byref(self.desc)
+        desc = KvCacheDesc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads, page, dim, code)
+        self.__dict__.update(k=k, v=v, k_scale=k_scale, v_scale=v_scale, device=device, heads=heads, dim=dim, desc=desc,
+                             ref=ctypes.byref(desc))
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"KVCache: {name} stays as it was given")
 
     @classmethod
     def empty(cls, pages: int, kv_heads: int, page: int = 64, head_dim: int = 128, dtype=torch.int8, device=None):
@@ -69,6 +68,11 @@ def _call(cache, name, *args) -> None:
             status = getattr(lib(), name)(cache.ref, *args, stream)
     if status:
         check(status)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(tokens, batch, heads, kv_heads, dim, max_new) -> int:
+    return lib().h3q_kv_attention_workspace_size(tokens, batch, heads, kv_heads, dim, max_new)
 
 
 def _ints(name, t, cache, n):
@@ -152,7 +156,7 @@ def attention(q, cache: KVCache, page_table, lengths, starts=None, scale: float 
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if return_lse else None
     if starts is None and batch:
         max_new = tokens // batch
-    need = lib().h3q_kv_attention_workspace_size(tokens, batch, heads, cache.heads, dim, max_new)
+    need = _workspace_bytes(tokens, batch, heads, cache.heads, dim, max_new)
     if workspace is None or workspace.numel() < need:
         workspace = q.new_empty(need, dtype=torch.uint8)
     _call(cache, "h3q_kv_attention", q.data_ptr(), _KIND[q.dtype], qt, qh, tokens, heads, table, width, lp, sp, batch, max_new,

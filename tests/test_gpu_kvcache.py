@@ -515,6 +515,8 @@ def test_refusals(cuda):
         kvcache.read(cache, table, n, 2)
     with pytest.raises(h3q.H3QError):
         kvcache.read(cache, table, _i32([0, 1, 2], cuda), 2, torch.int8)
+    with pytest.raises(AttributeError):  # the checks were of the tensors that it holds
+        cache.k = cache.k.clone()
     with pytest.raises(h3q.H3QError):
         kvcache.KVCache(cache.k, cache.v, cache.k_scale.double(), cache.v_scale)
     with pytest.raises(h3q.H3QError):
