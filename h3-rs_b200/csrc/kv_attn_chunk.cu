@@ -20,12 +20,14 @@
 // that have keys with their running sum, and the CTAs take equal contiguous ranges of the tiles of all (slot, kv head)
 // in order, so no wave is left part full; an item cut between CTAs is joined from f32 parts in order.
 //
-// Measured (B200): 2048 new tokens of 2 sequences over 10240, 32 heads (8 kv heads) of 128, causal, e4m3: 630 us for 0.62
-// TFLOP, 0.98 PFLOP/s; 1000 over 32760, 40 heads, int8: 715 us for 0.67 TFLOP; up to 1500 of 6 sequences, 16 heads of 64, a window of
-// 1024: 81 us, where each stretch of about ten tiles pays its start and end.  What bounds it is a row tile's chain (scores out
-// of TMEM, maximum, 128 exponentials a thread, weights into TMEM, two products), about 4000 cycles of which the products are
-// 1024 and the exponentials 1024 at their rates, with two row tiles to overlap: the tensor cores work 37 % of the time, the
-// exponential units 37 %, the issue slots 33 %.  A third row tile has no room in TMEM (2 x (128 + 128) columns are all of it).
+// Measured (B200): 2048 new tokens of 2 sequences over 10240, 32 heads (8 kv heads) of 128, causal, e4m3: 620 us for 0.62
+// TFLOP, 1.0 PFLOP/s; 1000 over 32760, 40 heads, int8: 727 us for 0.67 TFLOP; up to 1500 of 6 sequences, 16 heads of 64, a
+// window of 1024: 80 us.  A stretch costs 2.1 to 2.4 us a tile and 10 to 16 us for its start and end: q in (by cp.async; loads
+// through the few KB that are left of L1 took three times as long, and the first case 643 us), the first scores, O out.  What
+// bounds it is a row tile's chain (scores out of TMEM, maximum, 128 exponentials a thread, weights into TMEM, two products),
+// about 4000 cycles of which the products are 1024 and the exponentials 1024 at their rates, with two row tiles to overlap: the
+// tensor cores work 37 % of the time, the exponential units 37 %, the issue slots 33 %.  A third row tile has no room in TMEM
+// (2 x (128 + 128) columns are all of it).
 // Tried, no faster: weights in shared memory, passes of 16 or 32 columns, the maximum in the weights' pass with a redo, the second
 // product on halves of the weights, a late start of the second softmax, other register splits, codes widened from registers.
 // Every wait is bounded: on time-out the CTA latches an error code, waits for its MMAs, frees TMEM and returns.
@@ -67,6 +69,11 @@ struct Cfg {
   static constexpr size_t SMEM = 1024 + OFF_BAR + NBAR * 8 + 16;
   static_assert(SMEM + 16 <= 232448, "shared memory exceeds the sm_100 per-CTA limit");
 };
+
+// 16 bytes from global memory, or zeros
+__device__ __forceinline__ void cp16_zfill(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
 
 // the K-major 128-byte-swizzle descriptor of shared memory at 16 * `lo` bytes
 __device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
@@ -609,59 +616,60 @@ __global__ void __launch_bounds__(THREADS, 1)
       {
         constexpr int LPQ = D / 8;  // 16-byte pieces of a row
         const uint32_t qtile = smem_u32(smem + g * C::Q_TILE) + quarter * 32 * 128;
-        const int64_t src = (int64_t)(s.s0 + token) * a.q_ts + (int64_t)(s.kvh * a.per + (s.r0 + (in ? r : 0)) % a.per) * a.q_hs;
-        const int ch = lane % LPQ;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint4 v[LPQ / 2];
-#pragma unroll
-          for (int i = 0; i < LPQ / 2; ++i) {
-            const int row = (half * (LPQ / 2) + i) * (32 / LPQ) + lane / LPQ;
-            const int64_t at = __shfl_sync(0xffffffffu, src, row) + ch * 8;
-            const bool there = __shfl_sync(0xffffffffu, (int)in, row);
-            v[i] = make_uint4(0, 0, 0, 0);
-            if (there && q_vec) {
-              v[i] = __ldg(reinterpret_cast<const uint4*>(a.q + at));
-            } else if (there) {
-              uint32_t e[4];
+        const int64_t src =
+            in ? (int64_t)(s.s0 + token) * a.q_ts + (int64_t)(s.kvh * a.per + (s.r0 + r) % a.per) * a.q_hs : -1;
+        const int ch = lane % LPQ, row0 = lane / LPQ;
+        auto place = [&](int row) { return qtile + row * 128 + (ch >> 3) * C::Q_SLAB + (((ch & 7) ^ (row & 7)) << 4); };
+        if (q_vec) {  // past L1, of which this much shared memory leaves little
+#pragma unroll 4
+          for (int i = 0; i < LPQ; ++i) {
+            const int row = i * (32 / LPQ) + row0;
+            const int64_t at = __shfl_sync(0xffffffffu, src, row);
+            cp16_zfill(place(row), a.q + (at < 0 ? 0 : at + ch * 8), at >= 0);
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < LPQ; ++i) {
+            const int64_t at = __shfl_sync(0xffffffffu, src, i * (32 / LPQ) + row0);
+            uint32_t e[4] = {0, 0, 0, 0};
+            if (at >= 0)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                e[k] = (uint32_t)__ldg(a.q + at + 2 * k) | ((uint32_t)__ldg(a.q + at + 2 * k + 1) << 16);
-              v[i] = make_uint4(e[0], e[1], e[2], e[3]);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < LPQ / 2; ++i) {
-            const int row = (half * (LPQ / 2) + i) * (32 / LPQ) + lane / LPQ;
-            sts128(qtile + row * 128 + (ch >> 3) * C::Q_SLAB + (((ch & 7) ^ (row & 7)) << 4), v[i].x, v[i].y, v[i].z, v[i].w);
+                e[k] = (uint32_t)__ldg(a.q + at + ch * 8 + 2 * k) | ((uint32_t)__ldg(a.q + at + ch * 8 + 2 * k + 1) << 16);
+            sts128(place(i * (32 / LPQ) + row0), e[0], e[1], e[2], e[3]);
           }
         }
         __syncwarp();
+        // (small loops here too: what runs once a stretch is fetched anew each time)
         const uint32_t sign = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-        if (a.kind == 2 || sign) {
-          uint32_t w[D / 2];
-#pragma unroll
+        auto piece = [&](int i) { return qrow + (i >> 3) * C::Q_SLAB + (((i & 7) ^ swz) << 4); };
+        if (a.kind == 2) {
+          float mx = 0.f, f;
+#pragma unroll 4
           for (int i = 0; i < LPQ; ++i) {
-            const uint4 v = lds128(qrow + (i >> 3) * C::Q_SLAB + (((i & 7) ^ swz) << 4));
-            w[4 * i] = v.x;
-            w[4 * i + 1] = v.y;
-            w[4 * i + 2] = v.z;
-            w[4 * i + 3] = v.w;
+            const uint4 v = lds128(piece(i));
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mx = max3f(mx, fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xffff0000u)));
           }
-          if (a.kind == 2) {
-            float mx = 0.f, f;
+          kv_row_scale(mx, f, c);
+#pragma unroll 4
+          for (int i = 0; i < LPQ; ++i) {
+            const uint4 v = lds128(piece(i));
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int i = 0; i < D / 2; ++i)
-              mx = max3f(mx, fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u)));
-            kv_row_scale(mx, f, c);
-#pragma unroll
-            for (int i = 0; i < D / 2; ++i)
-              w[i] = kv_pack_f16(__uint_as_float(w[i] << 16) * f, __uint_as_float(w[i] & 0xffff0000u) * f);
+            for (int k = 0; k < 4; ++k)
+              w[k] = kv_pack_f16(__uint_as_float(w[k] << 16) * f, __uint_as_float(w[k] & 0xffff0000u) * f) ^ sign;
+            sts128(piece(i), w[0], w[1], w[2], w[3]);
           }
-#pragma unroll
-          for (int i = 0; i < LPQ; ++i)
-            sts128(qrow + (i >> 3) * C::Q_SLAB + (((i & 7) ^ swz) << 4), w[4 * i] ^ sign, w[4 * i + 1] ^ sign,
-                   w[4 * i + 2] ^ sign, w[4 * i + 3] ^ sign);
+        } else if (sign) {
+#pragma unroll 4
+          for (int i = 0; i < LPQ; ++i) {
+            const uint4 v = lds128(piece(i));
+            sts128(piece(i), v.x ^ sign, v.y ^ sign, v.z ^ sign, v.w ^ sign);
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
