@@ -298,7 +298,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       constexpr uint32_t idq = idesc_f16(BM, BN, false);
       constexpr uint32_t idp = idesc_f16(BM, D, false);
       // shared-memory addresses in units of 16 bytes: a step in K of 16 columns is 2, of 64 a slab
-      // shared-memory addresses in units of 16 bytes: a step in K of 16 columns is 2, of 64 a slab
       const uint32_t q0 = smem_u32(smem) >> 4, kv0 = smem_u32(smem + C::OFF_KV) >> 4;
       uint32_t slot = 0, phase = 0;  // place in the ring
       uint32_t segs0 = 0, segs1 = 0, done0 = 0, done1 = 0;  // segments and tiles of each row tile
@@ -854,7 +853,7 @@ cudaError_t launch_chunk(KvAttnArgs a, const KvChunkWork& wk, int q_vec, int* er
   }
   kv_attn_list_kernel<<<1, 1024, 0, st>>>(a, wk);
   if (const cudaError_t e = cudaGetLastError()) return e;
-  a.workers = sm_count(dev);
+  a.workers = sm_count(dev) < kMaxWorkers ? sm_count(dev) : kMaxWorkers;
   kern<<<(unsigned)a.workers, THREADS, Cfg<D>::SMEM, st>>>(a, wk, q_vec, err);
   if (const cudaError_t e = cudaGetLastError()) return e;
   return launch_kv_attn_join(a, ROWS, st);

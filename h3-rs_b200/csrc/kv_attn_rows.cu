@@ -20,8 +20,8 @@
 //
 // Measured (B200; head dim 128, 8 kv heads): one token of 64 sequences of up to 16384, int8, 5 query heads to a kv head,
 // 1.2 GB: 224 us, 5.4 TB/s; one of a sequence of 131000, 268 MB: 57 us, 4.7 TB/s; five of 16 sequences of up to 4099
-// (25 rows), e4m3: 41 us.  The copies alone reach 6.1 TB/s in the first: what keeps the rest is the widening of codes (a third
-// of the ALU pipe, five instructions for four codes) and its latencies, with 12 warps a multiprocessor for their
+// (25 rows), e4m3: 41 us.  The copies alone reach 6.1 TB/s in the first: what keeps the rest is the widening of codes (five
+// instructions for four; the ALU pipe is busy 45 % of the time) and its latencies, with 12 warps a multiprocessor for their
 // registers.  Tried and slower: scores in two accumulator chains (spills), two steps at a time (spills), 14 warps.
 #include <cstdint>
 #include <cuda_runtime.h>
@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
     };
     auto issue = [&](int st, int page, uint32_t dst) {
       if ((uint32_t)page < pool && st < steps) {
-        const int64_t off = page * page_bytes + (int64_t)(((kvh << group_log2) + ((group0 + st * kWarps) & group_mask)) * (16 * D)) + lane * 16;
+        const int64_t off = page * page_bytes + lane * 16 +
+                            (int64_t)(((kvh << group_log2) + ((group0 + st * kWarps) & group_mask)) * (16 * D));
         const uint8_t* ks = a.c.k + off;
         const uint8_t* vs = a.c.v + off;
 #pragma unroll
@@ -696,7 +697,9 @@ __global__ void __launch_bounds__(256, 4) kv_attn_join_kernel(const KvAttnArgs a
 
 cudaError_t launch_kv_attn_join(const KvAttnArgs& a, int tile, cudaStream_t st) {
   if (a.workers > (tile == 256 ? kMaxWorkers : kMaxRowWorkers)) return cudaErrorInvalidValue;
-  const dim3 grid((unsigned)(a.workers + (a.slots + 255) / 256), (unsigned)(tile == 256 ? a.c.dim / 16 : tile / (1024 / a.c.dim) > 1 ? tile / (1024 / a.c.dim) : 1));
+  const int blocks = tile / (1024 / a.c.dim);  // of 256 threads with a 16-byte chunk each, for a tile's rows
+  const dim3 grid((unsigned)(a.workers + (a.slots + 255) / 256),
+                  (unsigned)(tile == 256 ? blocks / 4 : blocks > 1 ? blocks : 1));
 #define H3Q_KV_J(DD, TT)                                     \
   if (a.c.dim == DD && tile == TT) {                         \
     kv_attn_join_kernel<DD, TT><<<grid, 256, 0, st>>>(a);    \
@@ -722,7 +725,7 @@ cudaError_t launch_rows(KvAttnArgs a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     ready[dev] = true;
   }
-  a.workers = sm_count(dev) * C::kCtas;
+  a.workers = sm_count(dev) * C::kCtas < kMaxRowWorkers ? sm_count(dev) * C::kCtas : kMaxRowWorkers;
   kern<<<(unsigned)a.workers, C::kThreads, C::kSmem, st>>>(a);
   if (const cudaError_t e = cudaGetLastError()) return e;
   return launch_kv_attn_join(a, MT * 16, st);
