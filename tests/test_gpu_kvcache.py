@@ -204,6 +204,18 @@ def test_attention_many_sequences(cuda, new):
     run_attention(cuda, I8, HF, 1, 2, 64, 16, totals, news, seed=3, max_new=max(news))
 
 
+@pytest.mark.parametrize("new", [1, 5, 70])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_one_head_split_over_every_worker(cuda, new, dim):
+    run_attention(cuda, E4, BF, 1, 5, dim, 128, [50001], [new], seed=29)
+
+
+@pytest.mark.parametrize("new", [1, 4])
+def test_attention_of_short_sequences_beside_long_ones(cuda, new):
+    totals = [new + 37 * i % 211 for i in range(60)] + [9001] + [new] * 5
+    run_attention(cuda, I8, HF, 2, 8, 128, 16, totals, [new] * len(totals), seed=31)
+
+
 def test_attention_scores_of_any_size(cuda):
     """Scores up to several hundred: one key takes all the weight, and the running maximum moves often."""
     run_attention(cuda, I8, BF, 1, 4, 128, 64, [1500], [3], seed=5, scale=4.0)
