@@ -54,7 +54,7 @@ __device__ __forceinline__ bool kv_slot(const KvAttnArgs& a, int64_t slot, int b
   t.lo = t.hi = 0;
   if (n <= 0 || all <= a.row_lo || all > a.row_hi) return false;
   const int64_t r0 = (slot - (a.one ? b : kv_slot_base(a.s, b, a.per, tile, 1))) * tile;
-  if (r0 >= all) return false;
+  if (r0 < 0 || r0 >= all) return false;  // (below 0: a slot before a first sequence that does not begin at row 0)
   t.b = b;
   t.s0 = s0;
   t.n = n;

@@ -138,8 +138,9 @@ __device__ __forceinline__ bool write_page(const KvCache& c, const KvSeqs& s, co
                                            WritePage& w) {
   const int s0 = kv_start(s, b), n = kv_start(s, b + 1) - s0;
   const int64_t had = __ldg(past + b);
-  if (n <= 0) return false;
-  const int64_t i = (had >> c.page_log2) + (slot - kv_slot_base(s, b, 1, c.page, 2));
+  const int64_t nth = slot - kv_slot_base(s, b, 1, c.page, 2);
+  if (n <= 0 || nth < 0) return false;  // (below 0: a slot before a first sequence that does not begin at row 0)
+  const int64_t i = (had >> c.page_log2) + nth;
   const int64_t p0 = i << c.page_log2;
   if (p0 >= had + n) return false;  // (a place before 0 has no page, like one behind the table's end)
   w.page = kv_page(c, s, b, i);  // -1: the page is not there; its tokens are dropped
@@ -344,8 +345,9 @@ __global__ void __launch_bounds__(256)
   const int b = kv_slot_seq_warp(s, slot, 1, c.page, 2);
   const int s0 = kv_start(s, b), n = kv_start(s, b + 1) - s0;
   const int64_t from = first ? __ldg(first + b) : 0;
-  if (n <= 0) return;
-  const int64_t pi = (from >> c.page_log2) + (slot - kv_slot_base(s, b, 1, c.page, 2));
+  const int64_t nth = slot - kv_slot_base(s, b, 1, c.page, 2);
+  if (n <= 0 || nth < 0) return;
+  const int64_t pi = (from >> c.page_log2) + nth;
   const int64_t p0 = pi << c.page_log2;
   if (p0 >= from + n) return;
   const int lo = from > p0 ? (int)(from - p0) : 0;
