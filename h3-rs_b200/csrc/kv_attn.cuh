@@ -3,9 +3,15 @@
 //
 // With c = scale * log2(e) and keys j of page p, both scales leave the matrix products:
 //     t_j = c ks_p (q . kcode_j),   w_j = 2^(t_j + log2 vs_p - m),   m within 2^8 of the row's largest t_j + log2 vs_p
-//     O = sum_j w_j vcode_j,   l = sum_p (1 / vs_p) sum_{j in p} w_j,   out = O / l,   lse = ln 2 (m + log2 l)
+//     O = sum_j w_j vcode_j,   l = sum_p 2^(m - u - log2 vs_p) sum_{j in p} w_j = sum_j 2^(t_j - u)
+//     out = O 2^(m - u) / l,   lse = ln 2 (u + log2 l)
 // so K and V enter the tensor cores as their codes, which 16-bit floats hold exactly, and one scale a page is applied
-// in f32.  What is rounded is w (f16) and the output; m, l, the scores and O are f32.
+// in f32.  What is rounded is w (f16) and the output; m, u, l, the scores and O are f32.
+//
+// u is at most the row's largest t_j.  l has a reference of its own because scales of V may lie 2^220 apart (1e-30 of a page
+// of zeros, 2^121 of the largest values): below 2^-126 w is 0, and a key counts in l whatever its values are.  While a
+// page's factor 2^(m - u - log2 vs_p) is at most 2^kKvFar, w is 0 only for keys below 2^(kKvFar - 126) of the row's largest
+// 2^t, which l has no bits for; beyond it a kernel sums 2^(t_j - u) itself, and raises u to the largest t_j that it sees there.
 //
 // q enters as f16: an f16 input as it is; a bf16 row times a power of two that brings its largest element near 1, which
 // is exact but for elements below 2^-14 of the row's largest (their error is under 2^-25 of it).
@@ -32,11 +38,13 @@ struct KvAttnArgs {
   int one;                 // every sequence of this launch has one slot, its own index
   int64_t slots;
   // Items (a slot and kv head) are cut between workers (CTAs); worker w's parts are 2 w (its first segment) and 2 w + 1.
-  // A part is O of its rows, [rows][dim] (tiles of 16 and 32) or [dim / 4][rows][4] (tiles of 256), then (m, l) a row.
+  // A part is O of its rows, [rows][dim] (tiles of 16 and 32) or [dim / 4][rows][4] (tiles of 256), then (m, u, l, 0) a row.
   float* part;
   int4* meta;              // [workers]: slot, kv head, first part and parts of the item that w began and did not finish
   int workers;
 };
+constexpr float kKvFar = 80.f;           // log2 of a page's largest factor in l
+constexpr float kKvNoRef = -1e30f;       // u of a row without keys: finite, so that differences are numbers or -inf
 constexpr int kMaxWorkers = 256;         // of the chunk kernel: one a multiprocessor
 constexpr int kMaxRowWorkers = 512;      // of the row kernel: up to three
 
@@ -98,14 +106,23 @@ __device__ __forceinline__ void kv_row_scale(float mx, float& f, float& c) {
   }
 }
 
+// A row's statistics, and what its sums O become its output by: O * inv * half * half (2^(m - u) in two factors, as it may be
+// beyond a float where the product is not).  A row without keys: zeros; a NaN in l goes through.
+struct KvStat {
+  float m, u, l;
+  __device__ __forceinline__ float inv() const { return l > 0.f ? __fdiv_rn(1.f, l) : (l == 0.f ? 0.f : l); }
+  __device__ __forceinline__ float half() const { return kv_ex2(0.5f * (m - u)); }
+  __device__ __forceinline__ float lse() const { return l == 0.f ? -INFINITY : 0.6931471805599453f * (u + log2f(l)); }
+};
+
 // four columns (chunk ch) of output row ro, from the unnormalised sums and the row's statistics
-__device__ __forceinline__ void kv_put_row(const KvAttnArgs& a, int64_t ro, int ch, int dim, float4 o, float m, float l) {
-  const float inv = l > 0.f ? __fdiv_rn(1.f, l) : (l == 0.f ? 0.f : l);  // no key: zeros; a NaN goes through
+__device__ __forceinline__ void kv_put_row(const KvAttnArgs& a, int64_t ro, int ch, int dim, float4 o, const KvStat& e) {
+  const float inv = e.inv(), f = e.half();
   uint2 w;
-  w.x = kv_pack(o.x * inv, o.y * inv, a.kind);
-  w.y = kv_pack(o.z * inv, o.w * inv, a.kind);
+  w.x = kv_pack(o.x * inv * f * f, o.y * inv * f * f, a.kind);
+  w.y = kv_pack(o.z * inv * f * f, o.w * inv * f * f, a.kind);
   *reinterpret_cast<uint2*>(a.out + ro * dim + ch * 4) = w;
-  if (a.lse && ch == 0) a.lse[ro] = l == 0.f ? -INFINITY : 0.6931471805599453f * (m + log2f(l));
+  if (a.lse && ch == 0) a.lse[ro] = e.lse();
 }
 
 // joins the parts of items that were cut between CTAs, and writes the rows of slots without keys

@@ -211,13 +211,44 @@ __device__ __forceinline__ bool next_segment(const KvAttnArgs& a, const KvChunkW
 
 }  // namespace
 
+// A tile with a page whose values are far below others of the stretch: its keys may count in l and have no w, so the row's
+// 2^t of the whole tile are summed here, by themselves.  Scores at tS, keys a0 .. a1 - 1 of the tile seen; u and l in and out.
+// A call, so that the loop over tiles, whose instructions barely fit the cache, is not longer for what is rare (2048-token
+// chunk: 651 us, 672 in line).
+__device__ __noinline__ float2 far_sums(uint32_t tS, const float4* cs, int a0, int a1, float c, float u, float l) {
+#pragma unroll 1
+  for (int q = 0; q < 8; ++q) {
+    const float4 e = cs[q];
+    if (e.y == -INFINITY) continue;
+    uint32_t y[16];
+    tmem_ld_32x32b_x16(tS + 16 * q, y);
+    tmem_wait_ld();
+    const uint32_t bits = below(a1 - 16 * q) & ~below(a0 - 16 * q);
+    const float ce = fmaxf(c * e.x, 1e-37f);
+    float to = u;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      y[i] = bits >> i & 1 ? y[i] : 0xff800000u;
+      to = fmaxf(to, __uint_as_float(y[i]) * ce);
+    }
+    l *= kv_ex2(u - to);
+    u = to;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) l += kv_ex2(__fmaf_rn(__uint_as_float(y[i]), ce, -u));
+  }
+  return make_float2(u, l);
+}
+
 template <int D, int CODES>
 __global__ void __launch_bounds__(THREADS, 1)
     kv_attn_chunk_kernel(const KvAttnArgs a, const KvChunkWork wk, int q_vec, int* err) {
   using C = Cfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float4* consts = reinterpret_cast<float4*>(smem + C::OFF_SC);  // [WR][8]: k scale, log2 of the v scale, its inverse
+  // [WR][8]: k scale, log2 of the v scale (-inf where there is no page), the tile's largest v scale over it (0), and in .w
+  // the logarithm of that largest one (entries 1 ..; inf without a page, which makes the weights' factor in l 0) and how far
+  // the least is below the largest of the stretch until then (entry 0)
+  float4* consts = reinterpret_cast<float4*>(smem + C::OFF_SC);
   uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* kv_empty = kv_full + RING;
   uint64_t* rk_full = kv_empty + RING;
@@ -421,13 +452,23 @@ __global__ void __launch_bounds__(THREADS, 1)
         int64_t key = s.sl.lo + (int64_t)s.t0 * BN + (lane & 7) * 16;  // lane l + 8 does as lane l does
         auto page_at = [&](int64_t k) { return k < s.sl.hi ? kv_page(a.c, a.s, s.sl.b, k >> a.c.page_log2) : (int64_t)-1; };
         int64_t page_next = page_at(key);
+        float loudest = -INFINITY;
         for (int j = s.t0; j < s.t1; ++j, ++tile, key += BN) {
           const int64_t page = page_next, ph = page * a.c.kv_heads + s.kvh;
           float4 c = make_float4(0.f, -INFINITY, 0.f, 0.f);
           if (page >= 0) {
-            const float vs = fmaxf(__ldg(a.c.v_scale + ph), kKvScaleFloor);
-            c = make_float4(__ldg(a.c.k_scale + ph), kv_lg2(vs), __fdividef(1.f, vs), 0.f);
+            c.x = __ldg(a.c.k_scale + ph);
+            c.y = kv_lg2(fmaxf(__ldg(a.c.v_scale + ph), kKvScaleFloor));
           }
+          float least = page >= 0 ? c.y : INFINITY, most = c.y;
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) {
+            least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+          }
+          loudest = fmaxf(loudest, most);
+          if (page >= 0) c.z = kv_ex2(fminf(most - c.y, kKvFar));
+          c.w = lane == 0 ? loudest - least : most > -INFINITY ? most : INFINITY;
           if (j + 1 < s.t1) page_next = page_at(key + BN);
           const int64_t off = (ph * a.c.page + (key & (a.c.page - 1))) * D;  // of the lane's 16 keys' codes
           // entry tile - 8 is read once the decode warps may fill K of tile - 4: its ring slot held V of tile - 6, whose
@@ -684,7 +725,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int khi = (int)(hi < key_base ? 0 : (hi - key_base < span ? hi - key_base : span));
       // the tiles that every row of the warp sees whole
       const int full_lo = __reduce_max_sync(0xffffffffu, klo), full_hi = __reduce_min_sync(0xffffffffu, khi);
-      float m_used = -INFINITY, l = 0.f;
+      float m_used = -INFINITY, u_used = kKvNoRef, l = 0.f;
       for (int j = 0; j < n; ++j) {
         const uint32_t T = tile0 + j;
         // (the ring only after the scores: a group that sat out slots may not look at it before it has come to them)
@@ -702,6 +743,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int k0 = j * BN;
         const bool edge = k0 < full_lo || k0 + BN > full_hi;  // some row does not see the whole tile
         const int a0 = klo - k0, a1 = khi - k0;
+        const bool far = cs[0].w > kKvFar;  // (m - u is at most the stretch's largest log2 vs)
+        if (__builtin_expect(far, 0)) {
+          const float2 e = far_sums(tS, cs, a0, a1, c, u_used, l);
+          u_used = e.x;
+          l = e.y;
+        }
         uint32_t x[4][32];
 #pragma unroll
         for (int k = 0; k < 4; ++k) tmem_ld_32x32b_x32(tS + 32 * k, x[k]);
@@ -733,9 +780,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (move) {
           alpha = kv_ex2(m_used - mx);
           m_used = mx;
+          const float u = mx - cq[1].w;  // at most the t of the key that mx is of
+          const float to = fmaxf(u_used, u);
+          l *= kv_ex2(u_used - to);
+          u_used = to;
         }
-        l *= alpha;
         const float m = m_used == -INFINITY ? 0.f : m_used;
+        const float l_f = far ? 0.f : kv_ex2(m_used - u_used - cq[1].w);  // of the loudest page's weights in l
+        float sum = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           uint32_t w[16];
@@ -755,10 +807,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             float s0, s1;
             upk(la, s0, s1);
-            l = __fmaf_rn(s0 + s1, cs[q].z, l);
+            sum = __fmaf_rn(s0 + s1, cs[q].z, sum);
           }
           tmem_st_32x32b_x16(tS + 16 * k, w);
         }
+        l = __fmaf_rn(sum, l_f, l);
         // O_g holds every product before these scores
         if (j > 0 && __any_sync(0xffffffffu, move)) {
 #pragma unroll 1
@@ -784,8 +837,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         break;
       }
       tc_fence_after();
-      float* part = a.part + (int64_t)part_slot * ROWS * (D + 2);
-      const float inv = l > 0.f ? __fdiv_rn(1.f, l) : (l == 0.f ? 0.f : l);  // a NaN goes through
+      float* part = a.part + (int64_t)part_slot * ROWS * (D + 4);
+      const KvStat stat{m_used, u_used, l};
+      const float inv = stat.inv(), f = stat.half();
 #pragma unroll 1
       for (int k = 0; k < D / 32; ++k) {
         uint32_t o[32];
@@ -797,7 +851,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              w[e] = kv_pack(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv, a.kind);
+              w[e] = kv_pack(__uint_as_float(o[8 * i + 2 * e]) * inv * f * f, __uint_as_float(o[8 * i + 2 * e + 1]) * inv * f * f,
+                             a.kind);
             const int ch = 4 * k + i;
             sts128(qrow + (ch >> 3) * C::Q_SLAB + (((ch & 7) ^ swz) << 4), w[0], w[1], w[2], w[3]);
           }
@@ -822,8 +877,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();  // read before the next stretch's rows go there
       }
       if (in) {
-        if (!s.whole) *reinterpret_cast<float2*>(part + (int64_t)ROWS * D + 2 * r) = make_float2(m_used, l);
-        else if (a.lse) a.lse[ro] = l == 0.f ? -INFINITY : 0.6931471805599453f * (m_used + log2f(l));
+        if (!s.whole) *reinterpret_cast<float4*>(part + (int64_t)ROWS * D + 4 * r) = make_float4(m_used, u_used, l, 0.f);
+        else if (a.lse) a.lse[ro] = stat.lse();
       }
       tc_fence_before();  // the reads of O are ordered before the next segment's first product, through p_full
     }
@@ -861,7 +916,7 @@ cudaError_t launch_chunk(KvAttnArgs a, const KvChunkWork& wk, int q_vec, int* er
 
 }  // namespace
 
-size_t kv_attn_chunk_part_bytes(int dim) { return (size_t)kMaxWorkers * 2 * ROWS * (dim + 2) * 4; }
+size_t kv_attn_chunk_part_bytes(int dim) { return (size_t)kMaxWorkers * 2 * ROWS * (dim + 4) * 4; }
 size_t kv_attn_chunk_list_bytes(int64_t slots) { return 256 + (size_t)slots * sizeof(KvListed); }
 
 cudaError_t launch_kv_attn_chunk(const KvAttnArgs& a, void* list, int* err, cudaStream_t st) {

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Sched<kWarps> sc;
   __shared__ float row_c[TILE];                   // c of the row: scale * log2 e and the power of two taken out of q
-  __shared__ float2 ml[kWarps][TILE], ml_all[TILE];
+  __shared__ KvStat ml[kWarps][TILE], ml_all[TILE];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   uint8_t* ring = smem + warp * C::kRing;
   const uint32_t ring_u = smem_u32(ring);
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
     __syncthreads();
 
     float o_acc[MT][NT][4];
-    float m_run[MT][2], l_run[MT][2], cr[MT][2];
+    float m_run[MT][2], u_run[MT][2], l_run[MT][2], cr[MT][2];
     int rlo[MT][2], rhi[MT][2];  // the row's keys, relative to key0
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -293,6 +293,7 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
       for (int hf = 0; hf < 2; ++hf) {
         const int r = mt * 16 + hf * 8 + g;
         m_run[mt][hf] = -INFINITY;
+        u_run[mt][hf] = kKvNoRef;
         l_run[mt][hf] = 0.f;
         cr[mt][hf] = row_c[r];
         int64_t lo = 0, hi = 0;
@@ -369,12 +370,13 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
       }
 
       // ------------------------------------------------------------ weights
-      const float lv = kv_lg2(vs), iv = __fdividef(1.f, vs);
+      const float lv = kv_lg2(vs);
       const bool edge = rel < all_lo || rel + 16 > all_hi;
       uint32_t pa[MT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         float ck[2], tv[2][4];  // [row half][key]: t + log2 vs - m; before the first maximum (m = -inf) it is +inf
+        float to_l[2];          // log2 of the factor of the weights in l
         bool up = false;
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
@@ -389,9 +391,10 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
               if (key < rlo[mt][hf] || key >= rhi[mt][hf]) tv[hf][k4] = -INFINITY;
             }
           }
-          up |= fmaxf(max3f(tv[hf][0], tv[hf][1], tv[hf][2]), tv[hf][3]) > kMove;
+          to_l[hf] = (m_run[mt][hf] - u_run[mt][hf]) - lv;
+          up |= max3f(max3f(tv[hf][0], tv[hf][1], tv[hf][2]), tv[hf][3], to_l[hf] - (kKvFar - kMove)) > kMove;
         }
-        if (__any_sync(0xffffffffu, up)) {  // rare after the first steps: move the maximum of the rows that need it
+        if (__any_sync(0xffffffffu, up)) {  // rare after the first steps: move the references of the rows that need it
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
             float t[4], mx = -INFINITY;
@@ -402,10 +405,17 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
             }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            auto raise = [&](float u) {
+              if (u > u_run[mt][hf]) {
+                l_run[mt][hf] *= kv_ex2(u_run[mt][hf] - u);
+                u_run[mt][hf] = u;
+              }
+            };
             if (mx > m_run[mt][hf] + kMove) {
               const float f = kv_ex2(m_run[mt][hf] - mx);  // 0 from -inf
               m_run[mt][hf] = mx;
-              l_run[mt][hf] *= f;
+              raise(mx - lv);
+              to_l[hf] = (m_run[mt][hf] - u_run[mt][hf]) - lv;
 #pragma unroll
               for (int j = 0; j < NT; ++j) {
                 o_acc[mt][j][2 * hf] *= f;
@@ -414,6 +424,14 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
 #pragma unroll
               for (int k4 = 0; k4 < 4; ++k4) tv[hf][k4] = t[k4] - mx;
             }
+            if (to_l[hf] > kKvFar) {  // this page's values are far below the row's largest: its keys' 2^t by themselves
+              raise(mx - lv);
+#pragma unroll
+              for (int k4 = 0; k4 < 4; ++k4)
+                if (t[k4] != -INFINITY)
+                  l_run[mt][hf] += kv_ex2(__fmaf_rn(s[mt][k4 >> 1][hf * 2 + (k4 & 1)], ck[hf], -u_run[mt][hf]));
+              to_l[hf] = -INFINITY;
+            }
           }
         }
 #pragma unroll
@@ -421,7 +439,7 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
           float p[4];
 #pragma unroll
           for (int k4 = 0; k4 < 4; ++k4) p[k4] = kv_ex2(tv[hf][k4]);
-          l_run[mt][hf] = __fmaf_rn((p[0] + p[1]) + (p[2] + p[3]), iv, l_run[mt][hf]);
+          l_run[mt][hf] = __fmaf_rn((p[0] + p[1]) + (p[2] + p[3]), kv_ex2(to_l[hf]), l_run[mt][hf]);
           pa[mt][hf] = kv_pack_f16(p[0], p[1]);
           pa[mt][2 + hf] = kv_pack_f16(p[2], p[3]);
         }
@@ -477,7 +495,7 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
         float l = l_run[mt][hf];
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t4 == 0) ml[warp][mt * 16 + hf * 8 + g] = make_float2(m_run[mt][hf], l);
+        if (t4 == 0) ml[warp][mt * 16 + hf * 8 + g] = KvStat{m_run[mt][hf], u_run[mt][hf], l};
       }
     __syncthreads();
 #pragma unroll
@@ -487,7 +505,7 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
         const int r = mt * 16 + hf * 8 + g;
         float m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i) m = fmaxf(m, ml[i][r].x);
+        for (int i = 0; i < kWarps; ++i) m = fmaxf(m, ml[i][r].m);
         const float f = m_run[mt][hf] == -INFINITY ? 0.f : kv_ex2(m_run[mt][hf] - m);
         // lane t holds d = t (D / 4) .. of the row: columns 2t and 2t + 1 of the tiles
 #pragma unroll
@@ -505,23 +523,26 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
           }
       }
     if (threadIdx.x < TILE) {
-      float m = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) m = fmaxf(m, ml[k][threadIdx.x].x);
+      KvStat e{-INFINITY, kKvNoRef, 0.f};
 #pragma unroll
       for (int k = 0; k < kWarps; ++k) {
-        const float2 e = ml[k][threadIdx.x];
-        l += e.x == -INFINITY ? 0.f : e.y * kv_ex2(e.x - m);
+        e.m = fmaxf(e.m, ml[k][threadIdx.x].m);
+        e.u = fmaxf(e.u, ml[k][threadIdx.x].u);
       }
-      ml_all[threadIdx.x] = make_float2(m, l);
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) {
+        const KvStat x = ml[k][threadIdx.x];
+        e.l += x.m == -INFINITY ? 0.f : x.l * kv_ex2(x.u - e.u);
+      }
+      ml_all[threadIdx.x] = e;
     }
     __syncthreads();
     const int part_slot = (int)(w * 2 + (first_segment ? 0 : 1));
-    float* part = a.part + (int64_t)part_slot * TILE * (D + 2);
+    float* part = a.part + (int64_t)part_slot * TILE * (D + 4);
     for (int i = threadIdx.x; i < sl.rows * (D / 4); i += kThreads) {
       const int r = i / (D / 4), ch = i % (D / 4), tt = ch / (D / 16);
       const uint32_t o = (uint32_t)(r * D * 4 + ((ch ^ ((tt * 2 + (r & 1)) & 7)) << 4));
-      const float2 e = ml_all[r];
+      const KvStat e = ml_all[r];
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < kWarps; ++k) {
@@ -532,10 +553,10 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
         sum.w += v.w;
       }
       if (whole) {
-        kv_put_row(a, kv_row_out(a, sl, kvh, r), ch, D, sum, e.x, e.y);
+        kv_put_row(a, kv_row_out(a, sl, kvh, r), ch, D, sum, e);
       } else {
         *reinterpret_cast<float4*>(part + (int64_t)r * D + ch * 4) = sum;
-        if (ch == 0) *reinterpret_cast<float2*>(part + (int64_t)TILE * D + 2 * r) = e;
+        if (ch == 0) *reinterpret_cast<float4*>(part + (int64_t)TILE * D + 4 * r) = make_float4(e.m, e.u, e.l, 0.f);
       }
     }
     if (u0 == 0 && !whole && threadIdx.x == 0) {
@@ -581,7 +602,7 @@ __global__ void __launch_bounds__(256, 4) kv_attn_join_kernel(const KvAttnArgs a
   // rows of few parts, a small one few rows of, at times, hundreds
   constexpr int CH = D / 4, BY = 256 / CH, R = TILE == 256 ? 4 : 1, ROWS = BY * R, AT_ONCE = 8 / R;
   constexpr int LANES = TILE == 256 ? 8 : 32;  // that look at the statistics of a row's parts
-  __shared__ float2 ml[ROWS];
+  __shared__ KvStat ml[ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if ((int)blockIdx.x >= a.workers) {
     if (blockIdx.y > 0) return;
@@ -614,7 +635,7 @@ __global__ void __launch_bounds__(256, 4) kv_attn_join_kernel(const KvAttnArgs a
       for (int64_t i = lane; i < (int64_t)rows * a.c.kv_heads * CH; i += 32) {
         const int64_t row = i / CH;
         kv_put_row(a, kv_row_out(a, e, (int)(row / rows), (int)(row % rows)), (int)(i % CH), D, make_float4(0.f, 0.f, 0.f, 0.f),
-                   0.f, l);
+                   KvStat{0.f, 0.f, l});
       }
     }
     return;
@@ -630,29 +651,29 @@ __global__ void __launch_bounds__(256, 4) kv_attn_join_kernel(const KvAttnArgs a
   KvSlot sl;
   if (!kv_slot(a, slot, b, TILE, sl)) return;
   // the first part is in the slot that its worker says, the others are their worker's first segment
-  auto part_of = [&](int i) { return a.part + (int64_t)(i == 0 ? meta.z : 2 * ((int)blockIdx.x + i)) * TILE * (D + 2); };
-  auto ml_of = [&](int i, int row) { return reinterpret_cast<const float2*>(part_of(i) + (int64_t)TILE * D) + row; };
+  auto part_of = [&](int i) { return a.part + (int64_t)(i == 0 ? meta.z : 2 * ((int)blockIdx.x + i)) * TILE * (D + 4); };
+  auto ml_of = [&](int i, int row) { return reinterpret_cast<const float4*>(part_of(i) + (int64_t)TILE * D) + row; };
   // neighbours in a warp are rows where the parts are [chunk][row] (tiles of 256), chunks where they are [row][chunk]
   const int tr = TILE == 256 ? threadIdx.x % BY : threadIdx.x / CH, ch = TILE == 256 ? threadIdx.x / BY : threadIdx.x % CH;
   for (int row0 = blockIdx.y * ROWS; row0 < sl.rows; row0 += gridDim.y * ROWS) {
     for (int r = threadIdx.x / LANES; r < ROWS; r += 256 / LANES) {
-      float m = -INFINITY, l = 0.f;
+      KvStat x{-INFINITY, kKvNoRef, 0.f};
       if (row0 + r < sl.rows)
         for (int i = lane % LANES; i < n; i += LANES) {
-          const float2 e = __ldg(ml_of(i, row0 + r));
-          const float to = fmaxf(m, e.x);
-          l *= m == -INFINITY ? 0.f : kv_ex2(m - to);
-          l = __fmaf_rn(e.x == -INFINITY ? 0.f : kv_ex2(e.x - to), e.y, l);
-          m = to;
+          const float4 e = __ldg(ml_of(i, row0 + r));
+          const float to = fmaxf(x.u, e.y);
+          x.l = __fmaf_rn(kv_ex2(e.y - to), e.z, x.l * kv_ex2(x.u - to));
+          x.u = to;
+          x.m = fmaxf(x.m, e.x);
         }
 #pragma unroll
       for (int o = LANES / 2; o; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o), to = fmaxf(m, m2);
-        const float f = m == -INFINITY ? 0.f : kv_ex2(m - to), f2 = m2 == -INFINITY ? 0.f : kv_ex2(m2 - to);
-        l = __fadd_rn(__fmul_rn(l, f), __fmul_rn(l2, f2));  // the same in both lanes
-        m = to;
+        const float u2 = __shfl_xor_sync(0xffffffffu, x.u, o), l2 = __shfl_xor_sync(0xffffffffu, x.l, o), to = fmaxf(x.u, u2);
+        x.l = __fadd_rn(__fmul_rn(x.l, kv_ex2(x.u - to)), __fmul_rn(l2, kv_ex2(u2 - to)));  // the same in both lanes
+        x.u = to;
+        x.m = fmaxf(x.m, __shfl_xor_sync(0xffffffffu, x.m, o));
       }
-      if (lane % LANES == 0) ml[r] = make_float2(m, l);
+      if (lane % LANES == 0) ml[r] = x;
     }
     __syncthreads();
     float4 o[R];
@@ -677,7 +698,7 @@ __global__ void __launch_bounds__(256, 4) kv_attn_join_kernel(const KvAttnArgs a
       for (int u = 0; u < AT_ONCE; ++u)
 #pragma unroll
         for (int k = 0; k < R; ++k) {
-          const float w = f[u][k] == -INFINITY ? 0.f : kv_ex2(f[u][k] - ml[tr + k * BY].x);
+          const float w = f[u][k] == -INFINITY ? 0.f : kv_ex2(f[u][k] - ml[tr + k * BY].m);
           if (w != 0.f) {  // a part that saw no key of the row may hold anything
             o[k].x = __fmaf_rn(v[u][k].x, w, o[k].x);
             o[k].y = __fmaf_rn(v[u][k].y, w, o[k].y);
@@ -689,7 +710,7 @@ __global__ void __launch_bounds__(256, 4) kv_attn_join_kernel(const KvAttnArgs a
 #pragma unroll
     for (int k = 0; k < R; ++k) {
       const int row = row0 + tr + k * BY;
-      if (row < sl.rows) kv_put_row(a, kv_row_out(a, sl, kvh, row), ch, D, o[k], ml[tr + k * BY].x, ml[tr + k * BY].y);
+      if (row < sl.rows) kv_put_row(a, kv_row_out(a, sl, kvh, row), ch, D, o[k], ml[tr + k * BY]);
     }
     __syncthreads();  // the statistics are read
   }
@@ -733,7 +754,7 @@ cudaError_t launch_rows(KvAttnArgs a, cudaStream_t st) {
 
 }  // namespace
 
-size_t kv_attn_rows_part_bytes(int dim, int tile) { return (size_t)kMaxRowWorkers * 2 * tile * (dim + 2) * 4; }
+size_t kv_attn_rows_part_bytes(int dim, int tile) { return (size_t)kMaxRowWorkers * 2 * tile * (dim + 4) * 4; }
 
 // tile: 16 or 32 rows
 cudaError_t launch_kv_attn_rows(const KvAttnArgs& a, int tile, cudaStream_t st) {

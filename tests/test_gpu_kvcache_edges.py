@@ -14,6 +14,44 @@ from test_gpu_kvcache import BF, E4, HF, I8, _gen, _i32, _starts, check_attentio
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("new,per,total", [(1, 4, 400), (8, 4, 400), (200, 1, 400), (1, 5, 30000), (70, 5, 30000)])
+@pytest.mark.parametrize("large", [1e12, 1e35])
+@pytest.mark.parametrize("score", [0.0, 1.0])
+def test_values_of_pages_far_apart(cuda, new, per, total, large, score):
+    """Pages of zeros at the smallest scale beside pages of values up to 1e37: each key counts in the denominator as its score
+    says, however small its values are beside others', and whichever worker or warp sees them."""
+    cache, table = make_cache(cuda, I8, 1, 16, 64, [total], 41)
+    ids = table[0, :-(-total // 16)].long()
+    cache.v_scale[ids[0::2]] = 1e-30
+    cache.v.view(torch.uint8)[ids[0::2]] = 0
+    cache.v_scale[ids[1::4]] = large
+    cache.v_scale[ids[: len(ids) // 3]] = 1e-30  # the first workers see nothing else
+    q = torch.randn((new, per, 64), generator=_gen(1, cuda), device=cuda).to(BF) * score
+    got, lse = kvcache.attention(q, cache, table, _i32([total], cuda), return_lse=True)
+    check_attention(q, cache, table, [total], [new], got, lse, 0.125, True, 0)
+    assert h3q.device_status() == 0
+
+
+@pytest.mark.parametrize("new", [5, 150])
+@pytest.mark.parametrize("window", [0, 300])
+def test_values_of_pages_far_apart_behind_masks(cuda, new, window):
+    """The same with windows that leave only quiet or only loud pages to a row, and stretches of pages that are not there."""
+    total, page = 3000, 32
+    cache, table = make_cache(cuda, E4, 2, page, 128, [total], 42)
+    ids = table[0, :-(-total // page)].long()
+    cache.v_scale[ids[0::3]] = 1e-30
+    cache.v_scale[ids[1::7]] = 1e25
+    cache.v_scale[ids[-4:]] = 1e-28  # what the newest rows see beside themselves is 2^170 louder
+    gone = [(320, 704), (2304, 2560), (2720, 2784)]
+    holes = table.clone()
+    for lo, hi in gone:
+        holes[0, lo // page:hi // page] = -1
+    q = torch.randn((new, 4, 128), generator=_gen(2, cuda), device=cuda).to(BF)
+    got, lse = kvcache.attention(q, cache, holes, _i32([total], cuda), window=window, return_lse=True)
+    check_attention(q, cache, table, [total], [new], got, lse, 128 ** -0.5, True, window, gone={0: gone})
+    assert h3q.device_status() == 0
+
+
 @pytest.mark.parametrize("first,news", [(16, [1, 1, 1, 1, 0]), (33, [40, 7]), (5, [200, 90]), (700, [150, 60])])
 def test_a_first_sequence_that_begins_behind_row_0(cuda, first, news):
     """Rows before starts[0] are nobody's: they are not written, and the others are as in a call without them.  Pages whose
