@@ -2,11 +2,14 @@
 // and keys of a slot, and the workspace that joins a slot's parts.
 //
 // With c = scale * log2(e) and keys j of page p, both scales leave the matrix products:
-//     t_j = c ks_p (q . kcode_j),   w_j = 2^(t_j + log2 vs_p - m),   m within 2^8 of the row's largest t_j + log2 vs_p
+//     t_j = c ks_p (q . kcode_j),   w_j = 2^(t_j + log2 vs_p - m),   the largest w of a row between 2^7 and 2^15
 //     O = sum_j w_j vcode_j,   l = sum_p 2^(m - u - log2 vs_p) sum_{j in p} w_j = sum_j 2^(t_j - u)
 //     out = O 2^(m - u) / l,   lse = ln 2 (u + log2 l)
 // so K and V enter the tensor cores as their codes, which 16-bit floats hold exactly, and one scale a page is applied
-// in f32.  What is rounded is w (f16) and the output; m, u, l, the scores and O are f32.
+// in f32.  What is rounded is w (f16) and the output; m, u, l, the scores and O are f32.  m starts 7 below the largest t_j +
+// log2 vs_p and moves when a w would pass 2^15: f16 has 11 bits of a weight down to 2^-21 of the largest and drops those below
+// 2^-32 of it, so that what a key of nearly all the weight leaves to tens of thousands of others still adds up (with the
+// largest at 1, 12800 equal keys with a hundredth of the weight between them lost 2 % of it).
 //
 // u is at most the row's largest t_j.  l has a reference of its own because scales of V may lie 2^220 apart (1e-30 of a page
 // of zeros, 2^121 of the largest values): below 2^-126 w is 0, and a key counts in l whatever its values are.  While a
@@ -43,6 +46,8 @@ struct KvAttnArgs {
   int4* meta;              // [workers]: slot, kv head, first part and parts of the item that w began and did not finish
   int workers;
 };
+constexpr float kKvTop = 15.f;           // log2 of the largest weight: f16 ends at 2^16
+constexpr float kKvLift = 7.f;           // log2 of the largest weight where m is set
 constexpr float kKvFar = 80.f;           // log2 of a page's largest factor in l
 constexpr float kKvNoRef = -1e30f;       // u of a row without keys: finite, so that differences are numbers or -inf
 constexpr int kMaxWorkers = 256;         // of the chunk kernel: one a multiprocessor

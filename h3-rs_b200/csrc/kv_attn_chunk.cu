@@ -8,7 +8,7 @@
 //   warps 4-11   softmax of tile 0 and 1: thread = row = TMEM lane; scales, maximum, W = 2^(t - m) as f16 back into TMEM
 //                over the scores it came from (the A operand of the second product is read from there: with W in
 //                shared memory the products alone would take the SM's whole shared-memory bandwidth), row sums; the
-//                maximum moves only when a tile raises it by more than 2^8;
+//                reference moves only when a weight would pass 2^15;
 //   warp 1       walks the work ahead of them: which rows and keys come next and, from the page table, the scales of each
 //                16 keys go into rings in shared memory, and the codes of two tiles ahead are copied there (cp.async.bulk),
 //                so that the others never wait for a length, a table entry or memory;
@@ -48,7 +48,6 @@ constexpr int RING = 3, RAW = 2, WR = 8;
 constexpr int REGS_MMA = 48, REGS_SOFT = 192, REGS_DEC = 80;
 static_assert(REGS_MMA + 2 * REGS_SOFT + REGS_DEC <= 4 * 128, "setmaxnreg split exceeds the launch");
 constexpr uint32_t TMEM_COLS = 512;
-constexpr float kMove = 8.f;
 
 template <int D>
 struct Cfg {
@@ -775,11 +774,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           cq[q].x = fmaxf(c * cq[q].x, 1e-37f);
           mx = fmaxf(mx, __fmaf_rn(fmaxf(max3f(u0, u1, u2), max3f(u3, u4, f(15))), cq[q].x, cq[q].y));
         }
-        const bool move = mx > m_used + kMove;
+        const bool move = mx > m_used + kKvTop;
         float alpha = 1.f;
         if (move) {
-          alpha = kv_ex2(m_used - mx);
-          m_used = mx;
+          alpha = kv_ex2(m_used - (mx - kKvLift));
+          m_used = mx - kKvLift;
           const float u = mx - cq[1].w;  // at most the t of the key that mx is of
           const float to = fmaxf(u_used, u);
           l *= kv_ex2(u_used - to);

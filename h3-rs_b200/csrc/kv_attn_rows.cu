@@ -32,8 +32,6 @@ namespace h3q {
 
 namespace {
 
-constexpr float kMove = 8.f;        // log2 of the largest weight between moves of the running maximum
-
 template <int D, int MT>
 struct RowsCfg {
   static constexpr int kWarps = 4, kThreads = kWarps * 32;
@@ -392,7 +390,7 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
             }
           }
           to_l[hf] = (m_run[mt][hf] - u_run[mt][hf]) - lv;
-          up |= max3f(max3f(tv[hf][0], tv[hf][1], tv[hf][2]), tv[hf][3], to_l[hf] - (kKvFar - kMove)) > kMove;
+          up |= max3f(max3f(tv[hf][0], tv[hf][1], tv[hf][2]), tv[hf][3], to_l[hf] - (kKvFar - kKvTop)) > kKvTop;
         }
         if (__any_sync(0xffffffffu, up)) {  // rare after the first steps: move the references of the rows that need it
 #pragma unroll
@@ -411,9 +409,9 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
                 u_run[mt][hf] = u;
               }
             };
-            if (mx > m_run[mt][hf] + kMove) {
-              const float f = kv_ex2(m_run[mt][hf] - mx);  // 0 from -inf
-              m_run[mt][hf] = mx;
+            if (mx > m_run[mt][hf] + kKvTop) {
+              const float m = mx - kKvLift, f = kv_ex2(m_run[mt][hf] - m);  // 0 from -inf
+              m_run[mt][hf] = m;
               raise(mx - lv);
               to_l[hf] = (m_run[mt][hf] - u_run[mt][hf]) - lv;
 #pragma unroll
@@ -422,7 +420,7 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
                 o_acc[mt][j][2 * hf + 1] *= f;
               }
 #pragma unroll
-              for (int k4 = 0; k4 < 4; ++k4) tv[hf][k4] = t[k4] - mx;
+              for (int k4 = 0; k4 < 4; ++k4) tv[hf][k4] = t[k4] - m;
             }
             if (to_l[hf] > kKvFar) {  // this page's values are far below the row's largest: its keys' 2^t by themselves
               raise(mx - lv);

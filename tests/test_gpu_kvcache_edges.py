@@ -52,6 +52,44 @@ def test_values_of_pages_far_apart_behind_masks(cuda, new, window):
     assert h3q.device_status() == 0
 
 
+@pytest.mark.parametrize("codes", [I8, E4])
+@pytest.mark.parametrize("new,per", [(1, 1), (5, 4), (40, 4)])
+def test_a_key_of_nearly_all_weight_and_no_value(cuda, codes, new, per):
+    """The first key has 0.99 of a row's weight and zeros for a value, so the row's output is the sum over the others, whose
+    weights are 2^-20 of the first's.  Weights are f16 times a power of two that brings the row's largest w to 2^7 or more, so
+    the smallest step is 2^-24 and a weight's rounding costs 2^-11 of it or 2^-25 of that power: 2^-32 max(p vs) sum |vcode|
+    in all; the other terms are those of check_attention."""
+    hk, dim, page, n, batch = 16, 64, 128, 12800, 24  # 384 rows of work share a pool: few of them are cut
+    g = _gen(7, cuda)
+    raw = [torch.zeros((n // page, hk, page, dim), device=cuda) for _ in range(2)]
+    raw[0][0, :, 0] = 100.0
+    raw[1].uniform_(60, 120, generator=g)
+    raw[1][0, :, 0] = 0
+    k, v = [(x.round() if codes == I8 else x).to(codes) for x in raw]
+    ks = torch.full((n // page, hk), 0.01, device=cuda)
+    vs = torch.full((n // page, hk), 0.02, device=cuda)
+    cache = kvcache.KVCache(k, v, ks, vs)
+    table = torch.arange(n // page, dtype=torch.int32, device=cuda).repeat(batch, 1)
+    q = torch.ones((batch * new, hk * per, dim), device=cuda).to(HF)  # q . k = 64 for the first key, 0 for the others
+    kfirst = float(k[0, 0, 0, 0].float())
+    scale = math.log(99.0 * n) / (64 * kfirst * float(ks[0, 0]))
+    got, lse = kvcache.attention(q, cache, table, _i32([n] * batch, cuda), scale=scale, return_lse=True)
+    scale = float(torch.tensor(scale, dtype=torch.float32))
+    vd = v.double().transpose(0, 1).flatten(1, 2) * float(vs[0, 0])  # [hk, n, dim]
+    first = math.exp(scale * 64 * kfirst * float(ks[0, 0]))
+    sums = vd.cumsum(1)
+    for i in range(new):
+        m = n - new + 1 + i  # keys that token i of a sequence sees
+        total = first + m - 1
+        want = sums[:, m - 1] / total
+        o = got.view(batch, new, hk, per, dim)[:, i].double()
+        sub = (first / total) * vd[:, :m].abs().sum(1)
+        tol = (2.0 ** -11 + 2.0 ** -16 + 2.0 ** -11) * want + 2.0 ** -32 * sub
+        worst = ((o - want[None, :, None]).abs() / tol[None, :, None]).max().item()
+        assert worst <= 1.0, (i, worst)
+        assert ((lse.view(batch, new, hk * per)[:, i].double() - math.log(total)).abs() <= 2.0 ** -17 * 20).all()
+
+
 @pytest.mark.parametrize("first,news", [(16, [1, 1, 1, 1, 0]), (33, [40, 7]), (5, [200, 90]), (700, [150, 60])])
 def test_a_first_sequence_that_begins_behind_row_0(cuda, first, news):
     """Rows before starts[0] are nobody's: they are not written, and the others are as in a call without them.  Pages whose
