@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int64_t page = page_next, ph = page * a.c.kv_heads + s.kvh;
           float4 c = make_float4(0.f, -INFINITY, 0.f, 0.f);
           if (page >= 0) {
-            c.x = __ldg(a.c.k_scale + ph);
+            c.x = fmaxf(__ldg(a.c.k_scale + ph), kKvScaleFloor);  // (the floor for a NaN)
             c.y = kv_lg2(fmaxf(__ldg(a.c.v_scale + ph), kKvScaleFloor));
           }
           float least = page >= 0 ? c.y : INFINITY, most = c.y;

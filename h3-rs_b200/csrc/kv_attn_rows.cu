@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
       issue(st + C::kStages - 1, pages[C::kStages - 1], put);
       next(put);
       const int page = pages[0];
-      const float ks = ks_next, vs = fmaxf(vs_next, kKvScaleFloor);
+      const float ks = fmaxf(ks_next, kKvScaleFloor), vs = fmaxf(vs_next, kKvScaleFloor);  // (the floor for a NaN)
 #pragma unroll
       for (int i = 0; i < C::kStages; ++i) pages[i] = pages[i + 1];
       pages[C::kStages] = entry_of(st + C::kStages + 1);

@@ -609,8 +609,8 @@ size_t h3q_kv_attention_workspace_size(int64_t tokens, int64_t batch, int64_t he
  * or NULL, receives the natural logarithm of the sum of exponentials (-inf for a row that sees no key).
  * max_new is an upper bound of the new tokens of one sequence (0: unknown); a tight one saves launches.  A sequence that
  * breaks it gets right results or, where no kernel of the call takes it, rows of NaN.
- * Scores, statistics and sums are f32; the weights enter the product with V as f16.  Scales below 1e-30 count as
- * 1e-30. */
+ * Scores, statistics and sums are f32; the weights enter the product with V as f16.  Scales of K and of V that are not at
+ * least 1e-30 (0, negative, NaN) count as 1e-30 here; h3q_kv_read multiplies by what is there. */
 h3q_status h3q_kv_attention(const h3q_kv_cache* cache, const void* q, int kind, int64_t q_token_stride,
                             int64_t q_head_stride, int64_t tokens, int64_t heads, const int32_t* page_table,
                             int64_t table_width, const int32_t* lengths, const int32_t* starts, int64_t batch,

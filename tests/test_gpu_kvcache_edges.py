@@ -90,6 +90,26 @@ def test_a_key_of_nearly_all_weight_and_no_value(cuda, codes, new, per):
         assert ((lse.view(batch, new, hk * per)[:, i].double() - math.log(total)).abs() <= 2.0 ** -17 * 20).all()
 
 
+@pytest.mark.parametrize("new", [1, 8, 200])
+def test_scales_below_the_smallest(cuda, new):
+    """Scales of 0, below 1e-30, negative and NaN count as 1e-30 in attention, those of K and of V alike, in every kernel."""
+    totals = [400]
+    bad, table = make_cache(cuda, I8, 2, 16, 128, totals, 13)
+    ids = table[0, :25].tolist()
+    good = kvcache.KVCache(bad.k, bad.v, bad.k_scale.clone(), bad.v_scale.clone())
+    for i, x in enumerate((0.0, 5e-31, -0.03, float("nan"), -math.inf)):
+        bad.k_scale[ids[2 * i]] = x
+        bad.v_scale[ids[2 * i + 11]] = x
+        good.k_scale[ids[2 * i]] = 1e-30
+        good.v_scale[ids[2 * i + 11]] = 1e-30
+    q = torch.randn((new, 8, 128), generator=_gen(1, cuda), device=cuda).to(BF)
+    n = _i32(totals, cuda)
+    want, want_lse = kvcache.attention(q, good, table, n, return_lse=True)
+    check_attention(q, good, table, totals, [new], want, want_lse, 128 ** -0.5, True, 0)
+    got, lse = kvcache.attention(q, bad, table, n, return_lse=True)
+    assert torch.equal(got, want) and torch.equal(lse, want_lse)
+
+
 @pytest.mark.parametrize("first,news", [(16, [1, 1, 1, 1, 0]), (33, [40, 7]), (5, [200, 90]), (700, [150, 60])])
 def test_a_first_sequence_that_begins_behind_row_0(cuda, first, news):
     """Rows before starts[0] are nobody's: they are not written, and the others are as in a call without them.  Pages whose
