@@ -53,11 +53,12 @@ constexpr float kKvNoRef = -1e30f;       // u of a row without keys: finite, so 
 constexpr int kMaxWorkers = 256;         // of the chunk kernel: one a multiprocessor
 constexpr int kMaxRowWorkers = 512;      // of the row kernel: up to three
 
-// What a slot stands for: `rows` query rows of sequence b, (token, head of the group) in that order, and the keys
-// [lo, hi) that any of them sees, lo a multiple of 16.
+// What a slot stands for: `rows` query rows of sequence b, (token, head of the group) in that order, the first of the
+// sequence's new tokens at place `first`, the tokens `len` that the table has room for, and the keys [lo, hi) that any of
+// the rows sees, lo a multiple of 16.
 struct KvSlot {
-  int b, s0, n, r0, rows;
-  int64_t len, lo, hi;
+  int b, s0, r0, rows;
+  int64_t first, len, lo, hi;
 };
 
 __device__ __forceinline__ bool kv_slot(const KvAttnArgs& a, int64_t slot, int b, int tile, KvSlot& t) {
@@ -70,14 +71,15 @@ __device__ __forceinline__ bool kv_slot(const KvAttnArgs& a, int64_t slot, int b
   if (r0 < 0 || r0 >= all) return false;  // (below 0: a slot before a first sequence that does not begin at row 0)
   t.b = b;
   t.s0 = s0;
-  t.n = n;
   t.r0 = (int)r0;
   t.rows = (int)(all - r0 < tile ? all - r0 : tile);
   int64_t len = __ldg(a.lengths + b);
+  len = len < 0 ? 0 : len;
+  t.first = len - n;
   const int64_t most = a.s.width << a.c.page_log2;
-  len = len < 0 ? 0 : (len > most ? most : len);
+  len = len > most ? most : len;  // what lies behind the table is not there; the queries keep their places
   t.len = len;
-  const int64_t first = len - n + t.r0 / a.per, last = len - n + (t.r0 + t.rows - 1) / a.per;
+  const int64_t first = t.first + t.r0 / a.per, last = t.first + (t.r0 + t.rows - 1) / a.per;
   int64_t hi = a.causal ? (last + 1 < len ? last + 1 : len) : len;
   int64_t lo = a.window > 0 && first + 1 > a.window ? first + 1 - a.window : 0;
   hi = hi < 0 ? 0 : hi;
@@ -88,7 +90,7 @@ __device__ __forceinline__ bool kv_slot(const KvAttnArgs& a, int64_t slot, int b
 
 // the keys [lo, hi) that row r of the slot sees
 __device__ __forceinline__ void kv_row_keys(const KvAttnArgs& a, const KvSlot& t, int r, int64_t& lo, int64_t& hi) {
-  const int64_t pos = t.len - t.n + (t.r0 + r) / a.per;
+  const int64_t pos = t.first + (t.r0 + r) / a.per;
   hi = a.causal && pos + 1 < t.len ? pos + 1 : t.len;
   lo = a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0;
 }

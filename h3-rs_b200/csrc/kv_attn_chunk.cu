@@ -179,9 +179,9 @@ namespace {
 // A stretch of tiles of one item, as the walker hands it to the other roles.
 struct Stretch {
   int rows, n;          // rows of the slot, tiles (0: the end)
-  int s0, r0, fresh;    // of the slot's sequence: first packed row, first row of the slot, new tokens
-  int kvh, whole, pad;
-  int64_t len, key_base;
+  int s0, r0;           // of the slot's sequence: first packed row, first row of the slot
+  int kvh, whole;
+  int64_t first, len, key_base;  // place of its first new token, tokens that the table has room for, first key
 };
 static_assert(sizeof(Stretch) == 48, "two of them in shared memory");
 
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           d.n = n;
           d.s0 = s.sl.s0;
           d.r0 = s.sl.r0;
-          d.fresh = s.sl.n;
+          d.first = s.sl.first;
           d.kvh = s.kvh;
           d.whole = s.t0 == 0 && s.t1 == s.e.tiles;
           d.len = s.sl.len;
@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (lane == 0) mbar_arrive(&q_full[g]);
       }
       // the keys of the row; a row that is not there sees all: its warp is spared the mask
-      const int64_t pos = s.len - s.fresh + token;
+      const int64_t pos = s.first + token;
       const int64_t key_base = s.key_base;
       const int64_t hi = in && a.causal && pos + 1 < s.len ? pos + 1 : s.len;
       const int64_t lo = in && a.window > 0 && pos + 1 > a.window ? pos + 1 - a.window : 0;

@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
       }
     }
     // keys of this segment that every row sees need no mask
-    const int64_t pos0 = sl.len - sl.n + sl.r0 / a.per, pos1 = sl.len - sl.n + (sl.r0 + sl.rows - 1) / a.per;
+    const int64_t pos0 = sl.first + sl.r0 / a.per, pos1 = sl.first + (sl.r0 + sl.rows - 1) / a.per;
     const int64_t all_hi64 = (a.causal && pos0 + 1 < sl.len ? pos0 + 1 : sl.len) - key0;
     const int64_t all_lo64 = (a.window > 0 && pos1 + 1 > a.window ? pos1 + 1 - a.window : 0) - key0;
     const int all_hi = (int)(all_hi64 < 0 ? 0 : (all_hi64 > 0x3fffffff ? 0x3fffffff : all_hi64));

@@ -110,6 +110,19 @@ def test_scales_below_the_smallest(cuda, new):
     assert torch.equal(got, want) and torch.equal(lse, want_lse)
 
 
+@pytest.mark.parametrize("new,causal,window", [(3, True, 0), (8, True, 0), (8, True, 40), (120, True, 0), (120, True, 50), (120, False, 0)])
+def test_a_table_shorter_than_the_sequence(cuda, new, causal, window):
+    """Tokens behind the table's last page are not there; the queries keep their positions, so masks stay where they were."""
+    totals = [170, 90]
+    cache, table = make_cache(cuda, I8, 2, 32, 64, totals, 14)
+    q = torch.randn((2 * new, 8, 64), generator=_gen(2, cuda), device=cuda).to(BF)
+    news = [new, new]
+    short = table[:, :3].contiguous()  # 96 tokens
+    got, lse = kvcache.attention(q, cache, short, _i32(totals, cuda), causal=causal, window=window, return_lse=True)
+    fixed = table.clamp_min(0)
+    check_attention(q, cache, fixed, totals, news, got, lse, 0.125, causal, window, gone={0: [(96, 170)]})
+
+
 @pytest.mark.parametrize("first,news", [(16, [1, 1, 1, 1, 0]), (33, [40, 7]), (5, [200, 90]), (700, [150, 60])])
 def test_a_first_sequence_that_begins_behind_row_0(cuda, first, news):
     """Rows before starts[0] are nobody's: they are not written, and the others are as in a call without them.  Pages whose
