@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
 #pragma unroll
       for (int k = 0; k < kWarps; ++k) {
         const KvStat x = ml[k][threadIdx.x];
-        e.l += x.m == -INFINITY ? 0.f : x.l * kv_ex2(x.u - e.u);
+        e.l += x.l * kv_ex2(x.u - e.u);  // (a warp without keys: 0; one whose every score is NaN: NaN)
       }
       ml_all[threadIdx.x] = e;
     }

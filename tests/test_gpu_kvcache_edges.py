@@ -123,6 +123,23 @@ def test_a_table_shorter_than_the_sequence(cuda, new, causal, window):
     check_attention(q, cache, fixed, totals, news, got, lse, 0.125, causal, window, gone={0: [(96, 170)]})
 
 
+@pytest.mark.parametrize("kind", [BF, HF])
+@pytest.mark.parametrize("new,total", [(1, 300), (1, 30000), (8, 300), (70, 300), (70, 30000)])
+def test_a_query_that_is_not_a_number(cuda, kind, new, total):
+    """A NaN in a query makes its row and its lse NaN, also where the row's keys are split between workers; the other rows
+    are what they are without it."""
+    cache, table = make_cache(cuda, I8, 1, 64, 64, [total], 15)
+    q = torch.randn((new, 4, 64), generator=_gen(3, cuda), device=cuda).to(kind)
+    n = _i32([total], cuda)
+    want, want_lse = kvcache.attention(q, cache, table, n, return_lse=True)
+    q[new // 2, 1, 5] = float("nan")
+    got, lse = kvcache.attention(q, cache, table, n, return_lse=True)
+    assert torch.isnan(got[new // 2, 1]).all() and torch.isnan(lse[new // 2, 1])
+    rest = torch.ones((new, 4), dtype=torch.bool, device=cuda)
+    rest[new // 2, 1] = False
+    assert torch.equal(got[rest], want[rest]) and torch.equal(lse[rest], want_lse[rest])
+
+
 @pytest.mark.parametrize("first,news", [(16, [1, 1, 1, 1, 0]), (33, [40, 7]), (5, [200, 90]), (700, [150, 60])])
 def test_a_first_sequence_that_begins_behind_row_0(cuda, first, news):
     """Rows before starts[0] are nobody's: they are not written, and the others are as in a call without them.  Pages whose
