@@ -590,7 +590,8 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
 // Block (w, y) of the first a.workers: rows of the item that worker w began and others went on with (at most one).  A
 // thread takes four columns of a row and adds the parts in their order, each with its factor 2^(m_i - m).  The blocks
 // after them look through the slots for those without any key, whose rows are zeros, and for sequences that no kernel of
-// the call takes, whose rows are NaN.
+// the call takes, whose rows are NaN.  Rows of no sequence are dealt to all blocks, and are zeros too (a call with starts
+// always has the launch for few rows, whose tiles are not 256).
 // Latency: 4 to 5 us for most calls of few rows, 11 us for a sequence of 131000 in 55 parts a kv head (14.5 us with four
 // loads in flight); 15 us for the 148 items of 256 rows of head dim 128 that a large chunk call cuts (23 us with a block for eight
 // rows instead of 32).
@@ -602,6 +603,14 @@ __global__ void __launch_bounds__(256, 4) kv_attn_join_kernel(const KvAttnArgs a
   constexpr int LANES = TILE == 256 ? 8 : 32;  // that look at the statistics of a row's parts
   __shared__ KvStat ml[ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (TILE != 256 && a.s.starts) {
+    const KvRest rest = kv_rest(a.s);
+    for (int i = blockIdx.x * gridDim.y + blockIdx.y; i < rest.n; i += gridDim.x * gridDim.y) {
+      const int64_t row = (int64_t)rest.row(i) * a.heads;
+      for (int k = threadIdx.x; k < a.heads * CH; k += 256)
+        kv_put_row(a, row + k / CH, k % CH, D, make_float4(0.f, 0.f, 0.f, 0.f), KvStat{0.f, 0.f, 0.f});
+    }
+  }
   if ((int)blockIdx.x >= a.workers) {
     if (blockIdx.y > 0) return;
     const int64_t slot0 = ((int64_t)(blockIdx.x - a.workers) * 8 + warp) * 32;

@@ -336,12 +336,22 @@ __global__ void __launch_bounds__(128)
   if (lane == 0) *scale = now;
 }
 
-// Rows of one page, all heads of a group: 16 codes (one 16-byte load) a thread and step.  OUT 0 f32, 1 f16, 2 bf16.
+// Rows of one page, all heads of a group: 16 codes (one 16-byte load) a thread and step.  OUT 0 f32, 1 f16, 2 bf16.  Rows of
+// no sequence are dealt to the blocks of a group of heads, and are zeros.
 template <int OUT, int CODES>
 __global__ void __launch_bounds__(256)
     kv_read_kernel(KvCache c, KvSeqs s, const int32_t* __restrict__ first, void* __restrict__ k_out,
                    void* __restrict__ v_out, int heads_each) {
   const int64_t slot = blockIdx.x;
+  const int h0 = blockIdx.y * heads_each, h1 = min(c.kv_heads, h0 + heads_each);
+  void* out = blockIdx.z ? v_out : k_out;
+  const KvRest rest = kv_rest(s);
+  for (int i = blockIdx.x; i < rest.n; i += gridDim.x) {
+    constexpr int size = OUT == 0 ? 4 : 2;
+    uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) +
+                                        ((int64_t)rest.row(i) * c.kv_heads + h0) * c.dim * size);
+    for (int k = threadIdx.x; k < (h1 - h0) * c.dim * size / 16; k += 256) d[k] = make_uint4(0, 0, 0, 0);
+  }
   const int b = kv_slot_seq_warp(s, slot, 1, c.page, 2);
   const int s0 = kv_start(s, b), n = kv_start(s, b + 1) - s0;
   const int64_t from = first ? __ldg(first + b) : 0;
@@ -354,10 +364,8 @@ __global__ void __launch_bounds__(256)
   const int hi = from + n - p0 < c.page ? (int)(from + n - p0) : c.page;
   const int64_t token0 = s0 + p0 - from;
   const int64_t page = kv_page(c, s, b, pi);
-  const int h0 = blockIdx.y * heads_each, h1 = min(c.kv_heads, h0 + heads_each);
   const uint8_t* codes = blockIdx.z ? c.v : c.k;
   const float* scale = blockIdx.z ? c.v_scale : c.k_scale;
-  void* out = blockIdx.z ? v_out : k_out;
   // The codes of the heads of a page follow one another, `page` rows each: vector v of the group is 16 codes of head
   // h0 + v / vectors_of_a_head, and every division is a shift.
   const int row_log2 = c.dim == 64 ? 2 : 3, head_log2 = c.page_log2 + row_log2;

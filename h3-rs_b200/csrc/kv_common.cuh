@@ -40,6 +40,20 @@ __device__ __forceinline__ int kv_start(const KvSeqs& s, int b) {
   return v < 0 ? 0 : (v > s.tokens ? s.tokens : v);
 }
 
+// The rows that belong to no sequence, before the first and behind the last: their number, and the i-th of them.
+struct KvRest {
+  int before, end, n;
+  __device__ __forceinline__ int row(int i) const { return i < before ? i : end + i - before; }
+};
+__device__ __forceinline__ KvRest kv_rest(const KvSeqs& s) {
+  KvRest r;
+  r.before = kv_start(s, 0);
+  r.end = kv_start(s, s.batch);
+  if (r.end < r.before) r.end = r.before;
+  r.n = r.before + s.tokens - r.end;
+  return r;
+}
+
 // page table[b, i], or -1 where the sequence has no such page
 __device__ __forceinline__ int64_t kv_page(const KvCache& c, const KvSeqs& s, int b, int64_t i) {
   if (i < 0 || i >= s.width) return -1;

@@ -8,8 +8,9 @@
 
 Page p of kv head h holds `page` tokens and one scale for K and one for V; value = code * scale.  Sequence b's tokens
 i * page .. are in page page_table[b, i].  The packed tokens of a call belong to its sequences by `starts` (int32
-[batch + 1], ascending from 0), or evenly without it.  page_table, past, lengths, first and starts are int32 CUDA tensors, which
-the host never reads.  Calls run on the current stream of the cache's device.
+[batch + 1], ascending; rows before starts[0] or from starts[-1] on are not written, and zeros in an output), or evenly
+without it.  page_table, past, lengths, first and starts are int32 CUDA tensors, which the host never reads.  Calls run on the
+current stream of the cache's device.
 """
 from __future__ import annotations
 

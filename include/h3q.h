@@ -563,10 +563,10 @@ h3q_status h3q_gemm_s8_static_status(int device, int* code);
  * of 16, 32, 64 or 128 tokens.
  *
  * The packed tokens of a call belong to its sequences by `starts` (int32 [batch + 1], ascending within 0 .. tokens;
- * a sequence may have none, and tokens before starts[0] or from starts[batch] on belong to nobody), or evenly where
- * starts is NULL.  page_table, past, lengths, first and starts are in
- * device memory and never read by the host: a call can be captured in a graph and replayed on other values.  Two
- * sequences may share a page that neither of them writes. */
+ * a sequence may have none, and tokens before starts[0] or from starts[batch] on belong to nobody: they are not written,
+ * and their rows of an output are zeros with an lse of -inf), or evenly where starts is NULL.  page_table, past,
+ * lengths, first and starts are in device memory and never read by the host: a call can be captured in a graph and
+ * replayed on other values.  Two sequences may share a page that neither of them writes. */
 enum { H3Q_KV_INT8 = 0, H3Q_KV_E4M3 = 1 };
 typedef struct h3q_kv_cache {
   void* k;

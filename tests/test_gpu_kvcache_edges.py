@@ -167,3 +167,41 @@ def test_a_first_sequence_that_begins_behind_row_0(cuda, first, news):
         want = kvcache.attention(q[first:], one, table, n, starts, max_new=most)
         assert torch.equal(want, kvcache.attention(q, one, table, n, late, max_new=most)[first:])
     assert h3q.device_status() == 0
+
+
+def _litter(*shapes):
+    """Leaves memory of these sizes full of NaN to the allocator."""
+    for shape, kind in shapes:
+        torch.full(shape, float("nan"), dtype=kind, device="cuda")
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("extra", [3, 700])
+def test_rows_of_no_sequence(cuda, new, extra):
+    """Rows behind the last sequence's (the padding of a captured step) or before the first are zeros, with an lse of -inf."""
+    totals, news = [100, 60], [new, new]
+    cache, table = make_cache(cuda, I8, 2, 32, 64, totals, 16)
+    t = 2 * new + extra
+    q = torch.randn((t, 8, 64), generator=_gen(4, cuda), device=cuda).to(BF)
+    n, starts = _i32(totals, cuda), _i32(_starts(news), cuda)
+    for most in (0, new):
+        _litter(((t, 8, 64), BF), ((t, 8), torch.float32))
+        got, lse = kvcache.attention(q, cache, table, n, starts, return_lse=True, max_new=most)
+        check_attention(q, cache, table, totals, news, got, lse, 0.125, True, 0)
+        assert (got[2 * new:] == 0).all() and (lse[2 * new:] == -math.inf).all()
+        _litter(((t, 8, 64), BF), ((t, 8), torch.float32))
+        late, late_lse = kvcache.attention(q, cache, table, n, starts + extra, return_lse=True, max_new=most)
+        check_attention(q[extra:], cache, table, totals, news, late[extra:], late_lse[extra:], 0.125, True, 0)
+        assert (late[:extra] == 0).all() and (late_lse[:extra] == -math.inf).all()
+    starts = _i32([0, 100, 160], cuda)
+    for kind in (torch.float32, HF, BF):
+        shape = (160 + extra, 2, 64)
+        _litter((shape, kind), (shape, kind))
+        k, v = kvcache.read(cache, table, starts, 160 + extra, kind)
+        want_k, want_v = kvcache.read(cache, table, starts, 160, kind)
+        assert torch.equal(k[:160], want_k) and torch.equal(v[:160], want_v)
+        assert (k[160:] == 0).all() and (v[160:] == 0).all()
+        _litter((shape, kind), (shape, kind))
+        k, v = kvcache.read(cache, table, starts + extra, 160 + extra, kind)
+        assert torch.equal(k[extra:], want_k) and torch.equal(v[extra:], want_v)
+        assert (k[:extra] == 0).all() and (v[:extra] == 0).all()
