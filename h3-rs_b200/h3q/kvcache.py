@@ -144,7 +144,8 @@ def attention(q, cache: KVCache, page_table, lengths, starts=None, scale: float 
     """softmax(scale * q . K) V of each sequence's newest tokens q [tokens, heads, head_dim] (f16 or bf16) over the first
     lengths [batch] tokens of its cache, the new ones included.  scale: head_dim ** -0.5 without it.  window > 0: the
     last `window` keys of each row.  max_new: an upper bound of the new tokens of one sequence, where starts is given and the
-    host knows one.  Returns [tokens, heads, head_dim], and with return_lse the f32 [tokens, heads] logarithms of the
+    host knows one.  workspace: a contiguous tensor of the cache's device that no other call uses meanwhile (a new one where it
+    is None or too small).  Returns [tokens, heads, head_dim], and with return_lse the f32 [tokens, heads] logarithms of the
     sums of exponentials."""
     if q.dtype != torch.bfloat16 and q.dtype != torch.float16:
         raise H3QError(ERR_ARG, "kvcache: q is f16 or bf16")
@@ -158,11 +159,14 @@ def attention(q, cache: KVCache, page_table, lengths, starts=None, scale: float 
     if starts is None and batch:
         max_new = tokens // batch
     need = _workspace_bytes(tokens, batch, heads, cache.heads, dim, max_new)
-    if workspace is None or workspace.numel() < need:
-        workspace = q.new_empty(need, dtype=torch.uint8)
+    if workspace is not None and (workspace.get_device() != cache.device or not workspace.is_contiguous()):
+        raise H3QError(ERR_ARG, "kvcache: the workspace is a contiguous tensor on the cache's device")
+    size = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    if workspace is None or size < need:
+        workspace, size = q.new_empty(need, dtype=torch.uint8), need
     _call(cache, "h3q_kv_attention", q.data_ptr(), _KIND[q.dtype], qt, qh, tokens, heads, table, width, lp, sp, batch, max_new,
           dim ** -0.5 if scale is None else scale, causal, window, out.data_ptr(), lse.data_ptr() if return_lse else None,
-          workspace.data_ptr(), workspace.numel())
+          workspace.data_ptr(), size)
     return (out, lse) if return_lse else out
 
 

@@ -205,3 +205,26 @@ def test_rows_of_no_sequence(cuda, new, extra):
         k, v = kvcache.read(cache, table, starts + extra, 160 + extra, kind)
         assert torch.equal(k[extra:], want_k) and torch.equal(v[extra:], want_v)
         assert (k[:extra] == 0).all() and (v[:extra] == 0).all()
+
+
+def test_workspaces(cuda):
+    """A workspace that the kernels could not write to is refused; one of any type is taken by its bytes, and a new one where
+    it is too small or has none."""
+    totals = [300, 20]
+    cache, table = make_cache(cuda, I8, 2, 32, 64, totals, 18)
+    q = torch.randn((80, 8, 64), generator=_gen(7, cuda), device=cuda).to(BF)
+    n = _i32(totals, cuda)
+    want = kvcache.attention(q, cache, table, n)
+    need = h3q.lib().h3q_kv_attention_workspace_size(80, 2, 8, 2, 64, 40)
+    for bad in (torch.empty(need, dtype=torch.uint8), torch.empty(2 * need, dtype=torch.uint8, device=cuda)[::2],
+                torch.empty(1, dtype=torch.uint8, device=cuda).expand(need), torch.empty(need, device="meta")):
+        with pytest.raises(h3q.H3QError) as e:
+            kvcache.attention(q, cache, table, n, workspace=bad)
+        assert e.value.status == h3q.ERR_ARG and "workspace" in str(e.value)
+    with pytest.raises(h3q.H3QError):  # not on a 16-byte boundary
+        kvcache.attention(q, cache, table, n, workspace=torch.empty(need + 1, dtype=torch.uint8, device=cuda)[1:])
+    guard = torch.full((need // 4 + 64,), 7.0, device=cuda)
+    for ws in (guard[:need // 4 + 1], torch.empty(16, dtype=torch.uint8, device=cuda),
+               torch.empty(0, dtype=torch.uint8, device=cuda), torch.empty(need, dtype=torch.uint8, device=cuda)):
+        assert torch.equal(kvcache.attention(q, cache, table, n, workspace=ws), want)
+    assert (guard[need // 4 + 1:] == 7).all()
