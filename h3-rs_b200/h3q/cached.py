@@ -17,7 +17,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import gemm_s8, kvcache, qk_norm_rope
+from . import ERR_ARG, H3QError, gemm_s8, kvcache, qk_norm_rope
 from .dit import Linear
 
 
@@ -35,27 +35,40 @@ class Layer:
 
 
 def positions(past, tokens: int, starts=None):
-    """The position of each packed token: past[b] + its place among its sequence's new ones."""
+    """The position of each packed token: past[b] + its place among its sequence's new ones.  A token of no sequence (before
+    starts[0] or from starts[-1] on) gets one that means nothing."""
+    batch = past.numel()
+    if batch == 0 and tokens > 0:
+        raise H3QError(ERR_ARG, "cached: tokens without a sequence")
     at = torch.arange(tokens, device=past.device, dtype=torch.int32)
     if starts is None:
-        each = tokens // past.numel()
-        return past.repeat_interleave(each, output_size=tokens) + at % each
-    seq = torch.searchsorted(starts[1:], at, right=True)
+        each = tokens // max(1, batch)
+        return past.repeat_interleave(each, output_size=tokens) + at % max(1, each)
+    seq = torch.searchsorted(starts[1:], at, right=True).clamp_(max=max(0, batch - 1))
     return past[seq] + at - starts[seq]
+
+
+def _rope_rows(rope, past, tokens: int, starts):
+    """The tokens' rows of rope.  Positions are values on the device, which nothing checks before they index: one outside of the
+    table takes its first or last row."""
+    if rope.dim() != 3 or rope.shape[0] != 2 or rope.shape[1] < 1:
+        raise H3QError(ERR_ARG, "cached: rope is [2, positions, rot / 2]")
+    return rope[:, positions(past, tokens, starts).clamp_(0, rope.shape[1] - 1).long()].contiguous()
 
 
 def attend(x, layer: Layer, cache: kvcache.KVCache, page_table, past, rope, starts=None, max_new: int = 0):
     """The layer on x bf16 [T, C], the new tokens of the sequences behind their past [batch] (int32) cached ones; rope f32
     [2, positions, rot / 2].  Writes the tokens' keys and values into the cache; returns bf16 [T, C].  The caller moves
-    past on after the last layer."""
+    past on after the last layer.  rope reaches as far as the sequences do: a token behind its end is rotated as its last
+    position, and one of no sequence (a captured step's padding) costs its row alone."""
     t, d, h, hk = x.shape[0], 128, layer.heads, layer.kv_heads
     qkv = gemm_s8(x, layer.qkv.w, layer.qkv.ws, layer.qkv.bias, rotate=True)
-    cs = rope[:, positions(past, t, starts).long()].contiguous()
+    cs = _rope_rows(rope, past, t, starts)
     q = qk_norm_rope(qkv, 0, h, d, (layer.q_norm, layer.eps), cs, layer.rot)
     k = qk_norm_rope(qkv, h * d, hk, d, (layer.k_norm, layer.eps), cs, layer.rot)
     v = qkv[:, (h + hk) * d:].unflatten(1, (hk, d))
     kvcache.write(cache, k, v, page_table, past, starts)
-    new = t // past.numel() if starts is None else starts[1:] - starts[:-1]
+    new = t // max(1, past.numel()) if starts is None else starts[1:] - starts[:-1]
     att = kvcache.attention(q, cache, page_table, past + new, starts, max_new=max_new)
     return gemm_s8(att.reshape(t, h * d), layer.out.w, layer.out.ws, layer.out.bias, rotate=True)
 
