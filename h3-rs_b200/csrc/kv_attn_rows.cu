@@ -590,11 +590,13 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
 // Block (w, y) of the first a.workers: rows of the item that worker w began and others went on with (at most one).  A
 // thread takes four columns of a row and adds the parts in their order, each with its factor 2^(m_i - m).  The blocks
 // after them look through the slots for those without any key, whose rows are zeros, and for sequences that no kernel of
-// the call takes, whose rows are NaN.  Rows of no sequence are dealt to all blocks, and are zeros too (a call with starts
-// always has the launch for few rows, whose tiles are not 256).
+// the call takes, whose rows are NaN.  The blocks after those, up to kRestBlocks of the launch for few rows of a call with starts
+// (which always has that launch), deal out the rows of no sequence, which are zeros too.  (Dealt to all blocks they cost a call
+// without any such row 0.9 us: two more loads ahead of every block's own.)
 // Latency: 4 to 5 us for most calls of few rows, 11 us for a sequence of 131000 in 55 parts a kv head (14.5 us with four
 // loads in flight); 15 us for the 148 items of 256 rows of head dim 128 that a large chunk call cuts (23 us with a block for eight
 // rows instead of 32).
+constexpr int kRestBlocks = 64;
 template <int D, int TILE>
 __global__ void __launch_bounds__(256, 4) kv_attn_join_kernel(const KvAttnArgs a) {
   // 16-byte chunks of a row; rows of a block, those of a thread BY apart; loads of a thread in flight: a large tile has many
@@ -603,15 +605,17 @@ __global__ void __launch_bounds__(256, 4) kv_attn_join_kernel(const KvAttnArgs a
   constexpr int LANES = TILE == 256 ? 8 : 32;  // that look at the statistics of a row's parts
   __shared__ KvStat ml[ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (TILE != 256 && a.s.starts) {
-    const KvRest rest = kv_rest(a.s);
-    for (int i = blockIdx.x * gridDim.y + blockIdx.y; i < rest.n; i += gridDim.x * gridDim.y) {
-      const int64_t row = (int64_t)rest.row(i) * a.heads;
-      for (int k = threadIdx.x; k < a.heads * CH; k += 256)
-        kv_put_row(a, row + k / CH, k % CH, D, make_float4(0.f, 0.f, 0.f, 0.f), KvStat{0.f, 0.f, 0.f});
-    }
-  }
   if ((int)blockIdx.x >= a.workers) {
+    const int first = a.workers + (int)((a.slots + 255) / 256);
+    if (TILE != 256 && (int)blockIdx.x >= first) {
+      const KvRest rest = kv_rest(a.s);
+      for (int i = (blockIdx.x - first) * gridDim.y + blockIdx.y; i < rest.n; i += (gridDim.x - first) * gridDim.y) {
+        const int64_t row = (int64_t)rest.row(i) * a.heads;
+        for (int k = threadIdx.x; k < a.heads * CH; k += 256)
+          kv_put_row(a, row + k / CH, k % CH, D, make_float4(0.f, 0.f, 0.f, 0.f), KvStat{0.f, 0.f, 0.f});
+      }
+      return;
+    }
     if (blockIdx.y > 0) return;
     const int64_t slot0 = ((int64_t)(blockIdx.x - a.workers) * 8 + warp) * 32;
     KvSlot t;
@@ -726,7 +730,8 @@ __global__ void __launch_bounds__(256, 4) kv_attn_join_kernel(const KvAttnArgs a
 cudaError_t launch_kv_attn_join(const KvAttnArgs& a, int tile, cudaStream_t st) {
   if (a.workers > (tile == 256 ? kMaxWorkers : kMaxRowWorkers)) return cudaErrorInvalidValue;
   const int blocks = tile / (1024 / a.c.dim);  // of 256 threads with a 16-byte chunk each, for a tile's rows
-  const dim3 grid((unsigned)(a.workers + (a.slots + 255) / 256),
+  const int rest = tile == 256 || !a.s.starts ? 0 : a.s.tokens < kRestBlocks ? a.s.tokens : kRestBlocks;
+  const dim3 grid((unsigned)(a.workers + (a.slots + 255) / 256 + rest),
                   (unsigned)(tile == 256 ? blocks / 4 : blocks > 1 ? blocks : 1));
 #define H3Q_KV_J(DD, TT)                                     \
   if (a.c.dim == DD && tile == TT) {                         \

@@ -346,13 +346,13 @@ __global__ void __launch_bounds__(256)
   const int h0 = blockIdx.y * heads_each, h1 = min(c.kv_heads, h0 + heads_each);
   void* out = blockIdx.z ? v_out : k_out;
   const KvRest rest = kv_rest(s);
+  const int b = kv_slot_seq_warp(s, slot, 1, c.page, 2);
   for (int i = blockIdx.x; i < rest.n; i += gridDim.x) {
     constexpr int size = OUT == 0 ? 4 : 2;
     uint4* d = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) +
                                         ((int64_t)rest.row(i) * c.kv_heads + h0) * c.dim * size);
     for (int k = threadIdx.x; k < (h1 - h0) * c.dim * size / 16; k += 256) d[k] = make_uint4(0, 0, 0, 0);
   }
-  const int b = kv_slot_seq_warp(s, slot, 1, c.page, 2);
   const int s0 = kv_start(s, b), n = kv_start(s, b + 1) - s0;
   const int64_t from = first ? __ldg(first + b) : 0;
   const int64_t nth = slot - kv_slot_base(s, b, 1, c.page, 2);

@@ -11,8 +11,8 @@ rotation), the projection's own bits for values.
 Output, in the 2-norm against attention over the history in 64 bits: rounding K and V moves a score by about its step over sqrt(12)
 and each weight with it, V by as much, independently over the keys, so the relative error is about sqrt(2 w) steps / sqrt(12) of
 unit values: page maxima near 4 give 0.009 (int8) and 0.036 (e4m3) a rounding, 0.026 and 0.1 for the four at most that
-a token sees here; the output linear quantises both sides' rows (3e-2, test_gpu_cached).  Held: 6e-2 and 1.5e-1.  A wrong column, norm, rotation or
-place moves it by about 1.
+a token sees here; the output linear quantises both sides' rows (3e-2, test_gpu_cached).  Held: 6e-2 and 1.5e-1; the other's norm moves it by
+0.12 to 0.15, a rotation one place on by 0.19, a column of the next head by 1.4, and each what the cache holds far beyond its bound.
 """
 import pytest
 import torch
