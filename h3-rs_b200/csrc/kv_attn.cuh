@@ -63,7 +63,7 @@ struct KvSlot {
 
 __device__ __forceinline__ bool kv_slot(const KvAttnArgs& a, int64_t slot, int b, int tile, KvSlot& t) {
   const int s0 = kv_start(a.s, b), n = kv_start(a.s, b + 1) - s0;
-  const int64_t all = (int64_t)n * a.per;  // at most 2^30 (checked by the host)
+  const int64_t all = (int64_t)n * a.per;  // beyond row_hi, which fits an int, only where a sequence breaks max_new
   t.rows = 0;
   t.lo = t.hi = 0;
   if (n <= 0 || all <= a.row_lo || all > a.row_hi) return false;

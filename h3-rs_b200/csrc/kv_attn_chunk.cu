@@ -20,15 +20,19 @@
 // that have keys with their running sum, and the CTAs take equal contiguous ranges of the tiles of all (slot, kv head)
 // in order, so no wave is left part full; an item cut between CTAs is joined from f32 parts in order.
 //
-// Measured (B200): 2048 new tokens of 2 sequences over 10240, 32 heads (8 kv heads) of 128, causal, e4m3: 620 us for 0.62
-// TFLOP, 1.0 PFLOP/s; 1000 over 32760, 40 heads, int8: 727 us for 0.67 TFLOP; up to 1500 of 6 sequences, 16 heads of 64, a
-// window of 1024: 80 us.  A stretch costs 2.1 to 2.4 us a tile and 10 to 16 us for its start and end: q in (by cp.async; loads
-// through the few KB that are left of L1 took three times as long, and the first case 643 us), the first scores, O out.  What
-// bounds it is a row tile's chain (scores out of TMEM, maximum, 128 exponentials a thread, weights into TMEM, two products),
-// about 4000 cycles of which the products are 1024 and the exponentials 1024 at their rates, with two row tiles to overlap: the
-// tensor cores work 37 % of the time, the exponential units 37 %, the issue slots 33 %.  A third row tile has no room in TMEM
-// (2 x (128 + 128) columns are all of it).
-// Tried, no faster: weights in shared memory, passes of 16 or 32 columns, the maximum in the weights' pass with a redo, the second
+// Measured (B200): 2048 new tokens of 2 sequences over 10240, 32 heads (8 kv heads) of 128, causal, e4m3: 645 us for 0.62
+// TFLOP, 0.96 PFLOP/s; 1000 over 32760, 40 heads, int8: 757 us for 0.67 TFLOP; up to 1500 of 6 sequences, 16 heads of 64, a
+// window of 1024: 86 us (617, 716 and 81 us before l had a reference of its own: the kernel is sensitive to a few more
+// instructions and registers in its loop).  A stretch costs 2.3 (head dim 64) to 2.9 us a tile and 12 to 14 us for its start and end: q in (by
+// cp.async; loads through the few KB that are left of L1 took three times as long, and 20 us more of the first case), the first
+// scores, O out.  What bounds it is a row tile's chain (scores out of TMEM, maximum, 128 exponentials a thread, weights
+// into TMEM, two products), about 4000 cycles of which the products are 1024 and the exponentials 1024 at their rates, with two
+// row tiles to overlap.  In a small case (1024 new tokens of one sequence over 6144, 127 us) the tensor cores work 36 % of the
+// time, the exponential units 37 %, the issue slots 34 %; by its flops the first case keeps the tensor cores busy for 42 % of
+// it at 1.9 GHz.  A third row tile has no room in TMEM at head dim 128 (2 x (128 + 128) columns are all of it); two threads a
+// row, and at head dim 64 the room that is left for a next stretch's q and outputs, are not tried.  156 bytes (168 there) of a
+// thread's registers are spilled.
+// Tried before that, no faster: weights in shared memory, passes of 16 or 32 columns, the maximum in the weights' pass with a redo, the second
 // product on halves of the weights, a late start of the second softmax, other register splits, codes widened from registers.
 // Every wait is bounded: on time-out the CTA latches an error code, waits for its MMAs, frees TMEM and returns.
 #include <cstdint>

@@ -19,8 +19,8 @@
 // six CTAs: 39.4, but 5 us more to join and 47.9 against 40.8 us for 25 rows).
 //
 // Measured (B200; head dim 128, 8 kv heads): one token of 64 sequences of up to 16384, int8, 5 query heads to a kv head,
-// 1.2 GB: 224 us, 5.4 TB/s; one of a sequence of 131000, 268 MB: 57 us, 4.7 TB/s; five of 16 sequences of up to 4099
-// (25 rows), e4m3: 41 us.  The copies alone reach 6.1 TB/s in the first: what keeps the rest is the widening of codes (five
+// 1.2 GB: 224 us, 5.4 TB/s; one of a sequence of 131000, 268 MB: 58 us, 4.6 TB/s; five of 16 sequences of up to 4099
+// (25 rows), e4m3: 42 us.  The copies alone reach 6.1 TB/s in the first: what keeps the rest is the widening of codes (five
 // instructions for four; the ALU pipe is busy 45 % of the time) and its latencies, with 12 warps a multiprocessor for their
 // registers.  Tried and slower: scores in two accumulator chains (spills), two steps at a time (spills), 14 warps.
 #include <cstdint>
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(RowsCfg<D, MT>::kThreads, RowsCfg<D, MT>::kCta
 // the call takes, whose rows are NaN.  The blocks after those, up to kRestBlocks of the launch for few rows of a call with starts
 // (which always has that launch), deal out the rows of no sequence, which are zeros too.  (Dealt to all blocks they cost a call
 // without any such row 0.9 us: two more loads ahead of every block's own.)
-// Latency: 4 to 5 us for most calls of few rows, 11 us for a sequence of 131000 in 55 parts a kv head (14.5 us with four
+// Latency: 4 to 6 us for most calls of few rows, 10 us for a sequence of 131000 in 55 parts a kv head (14.5 us with four
 // loads in flight); 15 us for the 148 items of 256 rows of head dim 128 that a large chunk call cuts (23 us with a block for eight
 // rows instead of 32).
 constexpr int kRestBlocks = 64;

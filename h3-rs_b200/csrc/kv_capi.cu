@@ -108,9 +108,11 @@ KvSeqs seqs_of(const int32_t* table, int64_t width, const int32_t* starts, int64
 
 // How a call's attention is cut: the row kernel takes the sequences of up to 32 query rows (new tokens times the query
 // heads of a kv head), the chunk kernel the others.  Each has its own part of the workspace.  Measured with their joins (int8, 8
-// kv heads of 128; 16 sequences of 4096 tokens / 64 of 1024): 16 rows 44 / 54 us as a tile of 16, 59 / 69 us as one of 32, 99 /
-// 144 us in the chunk kernel; 32 rows 65 / 80 us as a tile of 32, 101 / 146 us in the chunk kernel.  Beyond 32 rows a row tile's
-// accumulators no longer fit a warp's registers.
+// kv heads of 128; 16 sequences of 4096 tokens / 64 of 1024): 16 rows 44 / 54 us as a tile of 16, 59 / 69 us as one of 32, 104 /
+// 140 us in the chunk kernel; 32 rows 65 / 80 us as a tile of 32, 105 / 142 us in the chunk kernel.  Beyond 32 rows a row tile's
+// accumulators no longer fit a warp's registers.  The host knows no more than max_new: a call of ragged sequences without it is
+// planned for the worst, with tiles of 32 and the chunk kernel's launches (one token of 64 sequences of up to 16384, 40 heads:
+// 351 us in four kernels for 228 in two).
 struct AttnPlan {
   int tile;        // rows of a slot of the row kernel, 0: none of the sequences can be its
   int chunk;       // the chunk kernel runs

@@ -1,6 +1,8 @@
 """h3q.cached -- one attention layer of a text model that runs token by token or chunk by chunk: the library's linears and
 q / k RMSNorm + RoPE around the 8-bit key / value cache (h3q.kvcache).  The reference's text encoder sees its whole prompt at
-once (text.rs:377-395); this is the same layer with what came before kept in pages.
+once (text.rs:377-395); this is an attention layer of that kind, causal with shared kv heads, with what came before kept in
+pages.  Its linears are int8 ConvRot layers and its head dim is 128; the encoder's own NVFP4 + AWQ linears
+(h3q.nvfp4_linear) are not taken: a caller who has those makes the same calls around them.
 
     qkv = gemm_s8(x, qkv, rotate)                       [T, (heads + 2 kv_heads) * 128]
     q, k = qk_norm_rope(qkv columns, rope rows of the tokens' positions)

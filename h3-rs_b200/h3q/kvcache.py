@@ -143,10 +143,10 @@ def attention(q, cache: KVCache, page_table, lengths, starts=None, scale: float 
               window: int = 0, return_lse: bool = False, max_new: int = 0, workspace=None):
     """softmax(scale * q . K) V of each sequence's newest tokens q [tokens, heads, head_dim] (f16 or bf16) over the first
     lengths [batch] tokens of its cache, the new ones included.  scale: head_dim ** -0.5 without it.  window > 0: the
-    last `window` keys of each row.  max_new: an upper bound of the new tokens of one sequence, where starts is given and the
-    host knows one.  workspace: a contiguous tensor of the cache's device that no other call uses meanwhile (a new one where it
-    is None or too small).  Returns [tokens, heads, head_dim], and with return_lse the f32 [tokens, heads] logarithms of the
-    sums of exponentials."""
+    last `window` keys of each row.  max_new: an upper bound of the new tokens of one sequence, to be given with
+    starts (without it one token each of ragged sequences takes about half as long again).  workspace: a contiguous tensor
+    of the cache's device that no other call uses meanwhile (a new one where it is None or too small).  Returns [tokens,
+    heads, head_dim], and with return_lse the f32 [tokens, heads] logarithms of the sums of exponentials."""
     if q.dtype != torch.bfloat16 and q.dtype != torch.float16:
         raise H3QError(ERR_ARG, "kvcache: q is f16 or bf16")
     qt, qh = _rows("q", q, cache, q.shape[1] if q.dim() == 3 else 0)

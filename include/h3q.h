@@ -607,8 +607,9 @@ size_t h3q_kv_attention_workspace_size(int64_t tokens, int64_t batch, int64_t he
  * head h reads kv head h / (heads / kv_heads).  q is [tokens, heads, head_dim] of `kind` (f16 or bf16; strides in
  * elements, unit inside a head), out [tokens, heads, head_dim] of the same kind, contiguous; lse, f32 [tokens, heads]
  * or NULL, receives the natural logarithm of the sum of exponentials (-inf for a row that sees no key).
- * max_new is an upper bound of the new tokens of one sequence (0: unknown); a tight one saves launches.  A sequence that
- * breaks it gets right results or, where no kernel of the call takes it, rows of NaN.
+ * max_new is an upper bound of the new tokens of one sequence (0: unknown).  Give it with starts: without it one token each of
+ * ragged sequences takes about half as long again and ten times the workspace.  A sequence that breaks it gets right
+ * results or, where no kernel of the call takes it, rows of NaN.
  * Scores, statistics and sums are f32; the weights enter the product with V as f16.  Scales of K and of V that are not at
  * least 1e-30 (0, negative, NaN) count as 1e-30 here; h3q_kv_read multiplies by what is there. */
 h3q_status h3q_kv_attention(const h3q_kv_cache* cache, const void* q, int kind, int64_t q_token_stride,
