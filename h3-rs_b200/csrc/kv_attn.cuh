@@ -46,10 +46,10 @@ struct KvAttnArgs {
   int4* meta;              // [workers]: slot, kv head, first part and parts of the item that w began and did not finish
   int workers;
 };
-constexpr float kKvTop = 15.f;           // log2 of the largest weight: f16 ends at 2^16
+constexpr float kKvTop = 15.f;           // log2 of the largest weight: f16 ends at 2^16, room for the rounding of t up to 2^23
 constexpr float kKvLift = 7.f;           // log2 of the largest weight where m is set
 constexpr float kKvFar = 80.f;           // log2 of a page's largest factor in l
-constexpr float kKvNoRef = -1e30f;       // u of a row without keys: finite, so that differences are numbers or -inf
+constexpr float kKvNoRef = -3.402823466e38f;  // u of a row without keys: finite, so that differences are numbers or -inf
 constexpr int kMaxWorkers = 256;         // of the chunk kernel: one a multiprocessor
 constexpr int kMaxRowWorkers = 512;      // of the row kernel: up to three
 

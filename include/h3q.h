@@ -610,7 +610,8 @@ size_t h3q_kv_attention_workspace_size(int64_t tokens, int64_t batch, int64_t he
  * max_new is an upper bound of the new tokens of one sequence (0: unknown).  Give it with starts: without it one token each of
  * ragged sequences takes about half as long again and ten times the workspace.  A sequence that breaks it gets right
  * results or, where no kernel of the call takes it, rows of NaN.
- * Scores, statistics and sums are f32; the weights enter the product with V as f16.  Scales of K and of V that are not at
+ * Scores, statistics and sums are f32, so that scale * q . K beyond some 5e6 in magnitude, where f32 steps by whole units,
+ * says nothing and may come out as NaN; the weights enter the product with V as f16.  Scales of K and of V that are not at
  * least 1e-30 (0, negative, NaN) count as 1e-30 here; h3q_kv_read multiplies by what is there. */
 h3q_status h3q_kv_attention(const h3q_kv_cache* cache, const void* q, int kind, int64_t q_token_stride,
                             int64_t q_head_stride, int64_t tokens, int64_t heads, const int32_t* page_table,
